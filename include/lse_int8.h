@@ -368,6 +368,115 @@ int lse_paged_attention(const void *q, int dtype, int64_t H, int64_t D, int64_t 
                         int64_t max_q_len, float scale, void *o, int64_t o_stride_h, int64_t o_stride_m, void *stream);
 
 /*
+ * The 8-bit paged K/V cache.  Keys and values are int8 codes under one fp32 scale per page (a
+ * block of block_size consecutive positions) and KV head: value = code * scale.
+ *   k_pool, v_pool    int8 [num_blocks, H_kv, block_size, D], contiguous, 16-byte aligned (the
+ *                     page of one head is one contiguous run of block_size * D bytes)
+ *   k_scale, v_scale  fp32 [num_blocks, H_kv], contiguous
+ *   block_table       int32 [E, bt_cols], row stride bt_stride: position p of entry e is page
+ *                     block_table[e * bt_stride + p / block_size], slot p % block_size
+ * D = 64 or 128 and H / H_kv in {1, 2, 4, 8} (LSE_ERR_UNSUPPORTED otherwise), any block_size.
+ * It holds half the bytes of the bf16 pool that the reference allocates
+ * (src/llm_serving_engine/config.py:52-87), and takes the place of its K/V write
+ * (model_runner.py:342-355) and of paged_attention_forward (kernels/flash_attention.py:287-332).
+ *
+ * lse_kv8_rope_append -- rotate q and k of the fused QKV output and append k and v to the cache:
+ *   qkv       `dtype` (LSE_BF16 or LSE_F16) [M, (H + 2 H_kv) * D], row stride ld_qkv (a multiple
+ *             of 8), 16-byte aligned: q heads, then k heads, then v heads
+ *   cos, sin  [M, rotary_dim], row stride ld_cs, of cs_dtype (LSE_F32, LSE_BF16 or LSE_F16), one
+ *             value per rotated dim (both dims of a pair have theirs), so any frequency scaling
+ *             for long contexts is in the tables.  The first rotary_dim (even, 0 .. D) dims of
+ *             every q and k head rotate, x[d] cos[d] -+ x[partner] sin[d]: partner d +- rotary_dim/2
+ *             (interleaved = 0, rotate-half) or the other one of dims 2i, 2i + 1 (interleaved != 0);
+ *             the others pass.  rotary_dim = 0 needs no tables.
+ *   query_offset, q_start, q_len  int32 [E]: row q_start[e] + i (i < q_len[e]) of qkv is position
+ *             query_offset[e] + i of entry e
+ *   q_out     rotated q, `dtype` [H, M, D], contiguous, 16-byte aligned, every row of qkv
+ * A page that holds positions of earlier calls (query_offset inside it) keeps them: with s_old its
+ * scale (0 for a page whose first slot is new) and x the rows that this call puts into it,
+ *   s = max(s_old, max|x| / 127), earlier codes become rint(code * (s_old / s)) where s > s_old,
+ *   new codes are clamp(rint(x / s), -127, 127)
+ * in fp32; a page of zeros has scale 0.  A NaN or an infinity among x (or a NaN s_old) makes s NaN
+ * and the new codes 0: every value of that page and head reads as NaN until its first slot is
+ * written again.  No two entries of one call may append to the same page.  A page that is outside
+ * [0, num_blocks) or past bt_cols, and rows outside [0, M), are skipped and reported as
+ * LSE_ERR_INVALID_ARG by lse_device_status; an entry with q_len <= 0 appends nothing.
+ */
+int lse_kv8_rope_append(const void *qkv, int dtype, int64_t M, int64_t ld_qkv, int64_t H, int64_t H_kv, int64_t D,
+                        const void *cos, const void *sin, int64_t ld_cs, int cs_dtype, int64_t rotary_dim,
+                        int interleaved, void *q_out, int8_t *k_pool, int8_t *v_pool, float *k_scale, float *v_scale,
+                        int64_t num_blocks, int64_t block_size, const int32_t *block_table, int64_t bt_stride,
+                        int64_t bt_cols, const int32_t *query_offset, const int32_t *q_start, const int32_t *q_len,
+                        int64_t E, void *stream);
+
+/*
+ * Values of the pages block_ids[0 .. n) (int64) of one pool: out [n, H_kv, block_size, D] of
+ * `dtype` (LSE_BF16 or LSE_F16), contiguous, 16-byte aligned, code * scale rounded once.  An id
+ * outside [0, num_blocks) gives zeros and LSE_ERR_INVALID_ARG in lse_device_status.
+ */
+int lse_kv8_read(const int8_t *pool, const float *scale, int64_t num_blocks, int64_t block_size, int64_t H_kv, int64_t D,
+                 const int64_t *block_ids, int64_t n, void *out, int dtype, void *stream);
+
+/*
+ * Decode attention over the 8-bit cache, one query token per entry:
+ *   o[e, h, :] = softmax_p( q[e, h, :] . K[e, p, h / G, :] * scale ) V[e, p, h / G, :],
+ *                p = 0 .. context_len[e] - 1,  G = H / H_kv
+ *   q, o        `dtype`, element (e, h, d) at e * stride_e + h * stride_h + d, strides multiples
+ *               of 8, 16-byte aligned
+ *   context_len int32 [E]; above bt_cols * block_size it is cut there and reported as
+ *               LSE_ERR_INVALID_ARG by lse_device_status, as is a block id outside
+ *               [0, num_blocks), whose positions are masked and never read
+ *   workspace   >= lse_kv8_decode_attention_workspace(H, H_kv, D) bytes, 16-byte aligned, zeroed
+ *               once before its first use (every call leaves it ready for the next): any batch and
+ *               any context lengths, one buffer per stream
+ * fp32 scores, softmax and sums, one rounding of o.  An entry with nothing to attend to
+ * (context_len <= 0, or every page masked) gets zeros.
+ */
+size_t lse_kv8_decode_attention_workspace(int64_t H, int64_t H_kv, int64_t D);
+int lse_kv8_decode_attention(const void *q, int dtype, int64_t E, int64_t H, int64_t D, int64_t q_stride_e,
+                             int64_t q_stride_h, const int8_t *k_pool, const int8_t *v_pool, const float *k_scale,
+                             const float *v_scale, int64_t num_blocks, int64_t block_size, int64_t H_kv,
+                             const int32_t *block_table, int64_t bt_stride, int64_t bt_cols, const int32_t *context_len,
+                             float scale, void *o, int64_t o_stride_e, int64_t o_stride_h, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/*
+ * The same for any number of query tokens per entry (prompts, prompt chunks, mixed batches):
+ * q and o [H, tokens, D] (element (h, t, d) at h * stride_h + t * stride_m + d), entry e's rows
+ * q_start[e] .. q_start[e] + q_len[e] - 1, row i at position query_offset[e] + i, attending to the
+ * positions p < context_len[e] with p <= query_offset[e] + i.  Rows of no entry are not written;
+ * rows outside [0, tokens) are skipped and reported as LSE_ERR_INVALID_ARG by lse_device_status.
+ * Workspace as above, of lse_kv8_paged_attention_workspace(H, H_kv, D) bytes.
+ */
+size_t lse_kv8_paged_attention_workspace(int64_t H, int64_t H_kv, int64_t D);
+int lse_kv8_paged_attention(const void *q, int dtype, int64_t tokens, int64_t H, int64_t D, int64_t q_stride_h,
+                            int64_t q_stride_m, const int8_t *k_pool, const int8_t *v_pool, const float *k_scale,
+                            const float *v_scale, int64_t num_blocks, int64_t block_size, int64_t H_kv,
+                            const int32_t *block_table, int64_t bt_stride, int64_t bt_cols, const int32_t *context_len,
+                            const int32_t *query_offset, const int32_t *q_start, const int32_t *q_len, int64_t E,
+                            float scale, void *o, int64_t o_stride_h, int64_t o_stride_m, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
+/*
+ * Log-probabilities of rows of logits (the reference's sampler takes the same rows,
+ * src/llm_serving_engine/model/model_runner.py, and answers with tokens alone):
+ *   Z = sum_v exp(x[v] - max x);  logprob = x[token] - max x - log Z
+ *   entropy = log Z - sum_v (x[v] - max x) exp(x[v] - max x) / Z
+ *   top_logprobs, top_ids: the top_k largest x, equal ones by index (lowest first)
+ *   logits   `dtype` (LSE_BF16, LSE_F16 or LSE_F32) [M, V], row stride ld (>= V), element aligned
+ *   tokens   int64 [M], or null for no logprob; one outside [0, V) gives NaN and
+ *            LSE_ERR_INVALID_ARG in lse_device_status
+ *   top_k    0 .. min(V, LSE_LOGPROBS_MAX_TOP); top_logprobs fp32 [M, top_k], top_ids int64
+ * fp32 throughout.  -inf logits have probability 0; a row with nothing above -inf has
+ * log-probabilities -inf and entropy 0; a row holding a NaN or +inf has NaN for all of them.
+ * NaN counts as the largest value in the order of the alternatives.
+ */
+#define LSE_LOGPROBS_MAX_TOP 128
+int lse_token_logprobs(const void *logits, int dtype, int64_t M, int64_t V, int64_t ld, const int64_t *tokens,
+                       int64_t top_k, float *logprob, float *entropy, float *top_logprobs, int64_t *top_ids,
+                       void *stream);
+
+/*
  * Wait limit of the tensor-core kernels on `device`, in SM clock cycles: a bounded mbarrier wait
  * for data (a copy, an MMA, a stage) that has not completed after this many cycles raises the
  * CTA's abort flag and records LSE_ERR_DEVICE_TIMEOUT (lse_device_status); the CTA then drains

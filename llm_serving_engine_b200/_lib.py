@@ -39,6 +39,7 @@ WS_COUNTER_BYTES = 65536
 NOALLOC_SCRATCH_BYTES = 16777216  # fixed scratch of lse_int8_linear_packed_noalloc, per device
 NOALLOC_MAX_M = 64
 GATE_UP_SILU_MAX_M = 16  # lse_int8_gate_up_silu_packed's token range (the decode kernel's)
+LOGPROBS_MAX_TOP = 128  # lse_token_logprobs' largest top_k
 ABI_VERSION = 1
 
 # Every symbol include/lse_int8.h declares, with its ctypes signature.
@@ -83,6 +84,16 @@ SIGNATURES = {
     "lse_set_wait_limit": ([_I32, ctypes.c_longlong], _I32),
     "lse_paged_attention": ([_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P,
                              _I64, _I64, ctypes.c_float, _P, _I64, _I64, _P], _I32),
+    "lse_kv8_rope_append": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I32, _I64, _I32, _P, _P, _P, _P, _P,
+                             _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P], _I32),
+    "lse_kv8_read": ([_P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I32, _P], _I32),
+    "lse_kv8_decode_attention_workspace": ([_I64, _I64, _I64], _SZ),
+    "lse_kv8_decode_attention": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64,
+                                  _I64, _P, ctypes.c_float, _P, _I64, _I64, _P, _SZ, _P], _I32),
+    "lse_kv8_paged_attention_workspace": ([_I64, _I64, _I64], _SZ),
+    "lse_kv8_paged_attention": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64,
+                                 _I64, _P, _P, _P, _P, _I64, ctypes.c_float, _P, _I64, _I64, _P, _SZ, _P], _I32),
+    "lse_token_logprobs": ([_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P], _I32),
     "lse_abi_version": ([], _I32),
 }
 

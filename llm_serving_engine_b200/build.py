@@ -1,9 +1,10 @@
 """In-tree build of the sm_100a CUDA library (liblse_int8.so) with nvcc, and of the torch
 operators over it (liblse_torch.so) with the host C++ compiler.
 
-`python -m llm_serving_engine_b200.build` (or `build()`) compiles
-`csrc/lse_int8.cu` into `llm_serving_engine_b200/_lib/liblse_int8.so`, a plain C-ABI shared
-library (static CUDA runtime, no torch, no link-time libcuda), then `csrc/torch_ops.cpp` into
+`python -m llm_serving_engine_b200.build` (or `build()`) compiles the translation units
+`csrc/*.cu` (side by side; an object newer than every file it read is kept) and links them into
+`llm_serving_engine_b200/_lib/liblse_int8.so`, a plain C-ABI shared library (static CUDA
+runtime, no torch, no link-time libcuda), then `csrc/torch_ops.cpp` into
 `_lib/liblse_torch.so` (the `lse::int8_linear` / `lse::gate_up_silu` operators, linked to the
 first by a relative run path).  Each build is skipped when its output is newer than every
 source and header it reads.
@@ -16,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -34,7 +36,7 @@ def nvcc_path() -> str:
 
 
 def _sources() -> list[str]:
-    files = glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
+    files = [f for ext in ("*.cu", "*.cuh", "*.h") for f in glob.glob(os.path.join(CSRC, ext))]
     files.append(os.path.join(REPO_DIR, "include", "lse_int8.h"))
     return files
 
@@ -50,14 +52,20 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     if not force and up_to_date():
         return LIB_PATH
     os.makedirs(OUT_DIR, exist_ok=True)
+    units = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
+    keep = not force and not extra  # objects of other options are not reused
+    with ThreadPoolExecutor(len(units)) as pool:
+        objects = list(pool.map(lambda u: _compile(u, keep, verbose, extra or []), units))
     tmp = LIB_PATH + ".tmp"
-    cmd = [
-        nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17",
-        "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
-        "-Xptxas", "-warn-spills",
-        "-I", os.path.join(REPO_DIR, "include"),
-        os.path.join(CSRC, "lse_int8.cu"), "-o", tmp,
-    ] + (extra or [])
+    _run([nvcc_path(), *ARCH_FLAGS, "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", *objects, "-o", tmp], verbose)
+    if extra:
+        for o in objects:
+            os.remove(o)
+    os.replace(tmp, LIB_PATH)
+    return LIB_PATH
+
+
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -65,8 +73,20 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     if verbose and (res.stdout or res.stderr):
         print(res.stdout, res.stderr, file=sys.stderr)
-    os.replace(tmp, LIB_PATH)
-    return LIB_PATH
+
+
+def _compile(unit: str, keep: bool, verbose: bool, extra: list[str]) -> str:
+    """The object file of one translation unit, compiled unless it is newer than all it read."""
+    obj = os.path.join(OUT_DIR, os.path.basename(unit)[:-3] + ".o")
+    dep = obj[:-2] + ".d"
+    if keep and os.path.exists(obj) and os.path.exists(dep):
+        names = open(dep).read().replace("\\\n", " ").split(":", 1)[1].split()
+        t = os.path.getmtime(obj)
+        if all(os.path.exists(f) and os.path.getmtime(f) <= t for f in names):
+            return obj
+    _run([nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-warn-spills",
+          "-I", os.path.join(REPO_DIR, "include"), "-MD", "-MF", dep, "-c", unit, "-o", obj, *extra], verbose)
+    return obj
 
 
 TORCH_LIB_PATH = os.path.join(OUT_DIR, "liblse_torch.so")

@@ -1,0 +1,27 @@
+// Host-side helpers shared by the library's translation units (defined in lse_int8.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace lse {
+namespace host {
+
+// The calling thread's current device, set up (lse_init's work); an lse_status.
+int current_device(int *dev);
+int num_sms(int dev);
+// Keeps `e` as the thread's lse_last_cuda_error text and returns LSE_ERR_CUDA.
+int cuda_error(cudaError_t e, const char *where);
+// A launch configuration with programmatic dependent launch, as every kernel here is launched.
+void launch_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&attr)[1], dim3 grid, dim3 block, size_t smem,
+                   cudaStream_t st);
+
+}  // namespace host
+
+// Reads this translation unit's device status word on the current device (and clears it when
+// `reset`): each unit has its own copy, lse_device_status reports the first that is set.
+cudaError_t kv8_device_status(int *status, bool reset);
+cudaError_t logprobs_device_status(int *status, bool reset);
+
+}  // namespace lse

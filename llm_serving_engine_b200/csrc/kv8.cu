@@ -1,0 +1,285 @@
+// C-ABI entry points of the 8-bit paged K/V cache (declared in include/lse_int8.h): append with
+// rotation, page read, decode attention and multi-token attention.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "../../include/lse_int8.h"
+#include "host.h"
+#include "kv8_append.cuh"
+#include "kv8_attn.cuh"
+
+namespace lse {
+
+cudaError_t kv8_device_status(int *status, bool reset) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_device_status, sizeof(int));
+    const int zero = LSE_OK;
+    if (e == cudaSuccess && reset) e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
+    return e;
+}
+
+namespace {
+
+bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Arguments that every entry on the cache shares.
+int check_cache(int64_t H, int64_t H_kv, int64_t D, const void *k_pool, const void *v_pool, const void *k_scale,
+                const void *v_scale, int64_t num_blocks, int64_t block_size) {
+    if (H <= 0 || H_kv <= 0 || D <= 0 || num_blocks <= 0 || block_size <= 0 || H % H_kv) return LSE_ERR_INVALID_ARG;
+    if (!k_pool || !v_pool || !k_scale || !v_scale) return LSE_ERR_INVALID_ARG;
+    const int64_t G = H / H_kv;
+    if ((D != 64 && D != 128) || (G != 1 && G != 2 && G != 4 && G != 8)) return LSE_ERR_UNSUPPORTED;
+    if (H > 65535 || block_size > 65536 || num_blocks > INT32_MAX / 2 || num_blocks * block_size > INT32_MAX / 2)
+        return LSE_ERR_UNSUPPORTED;
+    if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
+        return LSE_ERR_ALIGNMENT;
+    return LSE_OK;
+}
+
+int check_table(const int32_t *block_table, int64_t bt_stride, int64_t bt_cols, int64_t E, int64_t block_size) {
+    if (!block_table || bt_stride < 0 || bt_cols < 0) return LSE_ERR_INVALID_ARG;
+    if (E > 1 && bt_stride < bt_cols) return LSE_ERR_INVALID_ARG;
+    if (E > (1 << 20) || bt_cols > INT32_MAX / 2 || bt_cols * block_size > INT32_MAX / 2) return LSE_ERR_UNSUPPORTED;
+    if (!aligned(block_table, 4)) return LSE_ERR_ALIGNMENT;
+    return LSE_OK;
+}
+
+int finish(cudaError_t e, const char *where) {
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? LSE_OK : host::cuda_error(e, where);
+}
+
+template <typename T>
+int launch_append(kv8::AppendParams<T> &p, int sms, cudaStream_t st) {
+    const int64_t q_elems = static_cast<int64_t>(p.M) * p.H * p.D;
+    p.q_blocks = static_cast<int>(std::min<int64_t>((q_elems + kv8::APPEND_THREADS - 1) / kv8::APPEND_THREADS, 8LL * sms));
+    // an entry of n tokens touches at most n / block_size + 2 pages (fewer warps only loop more)
+    const int64_t pages = static_cast<int64_t>(p.M) / p.block_size + 2LL * p.E;
+    const int64_t kv = std::min<int64_t>((pages * p.H_kv * 2 + 7) / 8, 8LL * sms);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(p.q_blocks + kv)), dim3(kv8::APPEND_THREADS), 0, st);
+    return finish(cudaLaunchKernelEx(&cfg, kv8::append_kernel<T>, p), "kv8_rope_append launch");
+}
+
+template <typename T>
+int run_append(const void *qkv, int64_t M, int64_t ld_qkv, int64_t H, int64_t H_kv, int64_t D, const void *cos,
+               const void *sin, int64_t ld_cs, int cs_dtype, int64_t R, int interleaved, void *q_out, int8_t *k_pool,
+               int8_t *v_pool, float *k_scale, float *v_scale, int64_t num_blocks, int64_t block_size,
+               const int32_t *block_table, int64_t bt_stride, int64_t bt_cols, const int32_t *query_offset,
+               const int32_t *q_start, const int32_t *q_len, int64_t E, int sms, cudaStream_t st) {
+    kv8::AppendParams<T> p{};
+    p.qkv = static_cast<const T *>(qkv);
+    p.ld_qkv = ld_qkv;
+    p.cos = cos;
+    p.sin = sin;
+    p.ld_cs = ld_cs;
+    p.cs_type = cs_dtype == LSE_BF16 ? 1 : cs_dtype == LSE_F16 ? 2 : 0;
+    p.R = static_cast<int>(R);
+    p.interleaved = interleaved != 0;
+    p.q_out = static_cast<T *>(q_out);
+    p.pool[0] = k_pool;
+    p.pool[1] = v_pool;
+    p.scale[0] = k_scale;
+    p.scale[1] = v_scale;
+    p.block_table = block_table;
+    p.bt_stride = bt_stride;
+    p.bt_cols = static_cast<int>(bt_cols);
+    p.query_offset = query_offset;
+    p.q_start = q_start;
+    p.q_len = q_len;
+    p.M = static_cast<int>(M);
+    p.H = static_cast<int>(H);
+    p.H_kv = static_cast<int>(H_kv);
+    p.D = static_cast<int>(D);
+    p.E = static_cast<int>(E);
+    p.num_blocks = static_cast<int>(num_blocks);
+    p.block_size = static_cast<int>(block_size);
+    return launch_append(p, sms, st);
+}
+
+template <int D, typename T>
+int launch_rows(const kv8::AttnParams &p, int sms, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    const int64_t blocks = std::min<int64_t>((static_cast<int64_t>(p.tokens) * p.H + 7) / 8, 64LL * sms);
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st);
+    return finish(cudaLaunchKernelEx(&cfg, kv8::attn_rows_kernel<D, T>, p), "kv8 attention launch");
+}
+
+int launch_attention(const kv8::AttnParams &p, int dtype, int64_t D, int sms, cudaStream_t st) {
+    if (dtype == LSE_F16) return D == 128 ? launch_rows<128, __half>(p, sms, st) : launch_rows<64, __half>(p, sms, st);
+    return D == 128 ? launch_rows<128, __nv_bfloat16>(p, sms, st) : launch_rows<64, __nv_bfloat16>(p, sms, st);
+}
+
+}  // namespace
+}  // namespace lse
+
+using namespace lse;
+
+extern "C" {
+
+int lse_kv8_rope_append(const void *qkv, int dtype, int64_t M, int64_t ld_qkv, int64_t H, int64_t H_kv, int64_t D,
+                        const void *cos, const void *sin, int64_t ld_cs, int cs_dtype, int64_t rotary_dim,
+                        int interleaved, void *q_out, int8_t *k_pool, int8_t *v_pool, float *k_scale, float *v_scale,
+                        int64_t num_blocks, int64_t block_size, const int32_t *block_table, int64_t bt_stride,
+                        int64_t bt_cols, const int32_t *query_offset, const int32_t *q_start, const int32_t *q_len,
+                        int64_t E, void *stream) {
+    if (M < 0 || E < 0 || H_kv <= 0 || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1)) return LSE_ERR_INVALID_ARG;
+    if (dtype != LSE_BF16 && dtype != LSE_F16) return LSE_ERR_UNSUPPORTED;
+    if (M == 0) return LSE_OK;
+    int rc = check_cache(H, H_kv, D, k_pool, v_pool, k_scale, v_scale, num_blocks, block_size);
+    if (rc) return rc;
+    if (!qkv || !q_out || ld_qkv < (H + 2 * H_kv) * D) return LSE_ERR_INVALID_ARG;
+    if (rotary_dim) {
+        if (!cos || !sin || ld_cs < rotary_dim) return LSE_ERR_INVALID_ARG;
+        if (cs_dtype != LSE_F32 && cs_dtype != LSE_BF16 && cs_dtype != LSE_F16) return LSE_ERR_INVALID_ARG;
+        const uintptr_t n = cs_dtype == LSE_F32 ? 4 : 2;
+        if (!aligned(cos, n) || !aligned(sin, n)) return LSE_ERR_ALIGNMENT;
+    }
+    if (E && (!query_offset || !q_start || !q_len)) return LSE_ERR_INVALID_ARG;
+    if (E && (rc = check_table(block_table, bt_stride, bt_cols, E, block_size))) return rc;
+    if (M > INT32_MAX / 2) return LSE_ERR_UNSUPPORTED;
+    if (!aligned(qkv, 16) || !aligned(q_out, 16) || ld_qkv % 8) return LSE_ERR_ALIGNMENT;
+    int dev = 0;
+    if ((rc = host::current_device(&dev))) return rc;
+    const auto run = dtype == LSE_F16 ? run_append<__half> : run_append<__nv_bfloat16>;
+    return run(qkv, M, ld_qkv, H, H_kv, D, cos, sin, ld_cs, cs_dtype, rotary_dim, interleaved, q_out, k_pool, v_pool,
+               k_scale, v_scale, num_blocks, block_size, block_table, bt_stride, bt_cols, query_offset, q_start, q_len, E,
+               host::num_sms(dev), static_cast<cudaStream_t>(stream));
+}
+
+int lse_kv8_read(const int8_t *pool, const float *scale, int64_t num_blocks, int64_t block_size, int64_t H_kv, int64_t D,
+                 const int64_t *block_ids, int64_t n, void *out, int dtype, void *stream) {
+    if (num_blocks <= 0 || block_size <= 0 || H_kv <= 0 || D <= 0 || n < 0) return LSE_ERR_INVALID_ARG;
+    if (dtype != LSE_BF16 && dtype != LSE_F16) return LSE_ERR_UNSUPPORTED;
+    if (n == 0) return LSE_OK;
+    if (!pool || !scale || !block_ids || !out) return LSE_ERR_INVALID_ARG;
+    if (num_blocks > INT32_MAX / 2 || block_size * D > INT32_MAX / 2 || H_kv > 65535 || n > INT32_MAX / 2 || D % 16)
+        return LSE_ERR_UNSUPPORTED;
+    if (!aligned(pool, 16) || !aligned(out, 16) || !aligned(scale, 4) || !aligned(block_ids, 8)) return LSE_ERR_ALIGNMENT;
+    int dev = 0;
+    if (int rc = host::current_device(&dev)) return rc;
+    const int64_t total = n * H_kv * block_size * D;
+    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16LL * host::num_sms(dev));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<cudaStream_t>(stream));
+    const int nb = static_cast<int>(num_blocks), hk = static_cast<int>(H_kv), pe = static_cast<int>(block_size * D);
+    const cudaError_t e = dtype == LSE_F16
+        ? cudaLaunchKernelEx(&cfg, kv8::read_kernel<__half>, pool, scale, nb, hk, pe, block_ids, n, static_cast<__half *>(out))
+        : cudaLaunchKernelEx(&cfg, kv8::read_kernel<__nv_bfloat16>, pool, scale, nb, hk, pe, block_ids, n,
+                             static_cast<__nv_bfloat16 *>(out));
+    return finish(e, "kv8_read launch");
+}
+
+size_t lse_kv8_decode_attention_workspace(int64_t H, int64_t H_kv, int64_t D) {
+    (void)H;
+    (void)H_kv;
+    (void)D;
+    return 0;
+}
+
+int lse_kv8_decode_attention(const void *q, int dtype, int64_t E, int64_t H, int64_t D, int64_t q_stride_e,
+                             int64_t q_stride_h, const int8_t *k_pool, const int8_t *v_pool, const float *k_scale,
+                             const float *v_scale, int64_t num_blocks, int64_t block_size, int64_t H_kv,
+                             const int32_t *block_table, int64_t bt_stride, int64_t bt_cols, const int32_t *context_len,
+                             float scale, void *o, int64_t o_stride_e, int64_t o_stride_h, void *workspace,
+                             size_t workspace_bytes, void *stream) {
+    (void)workspace;
+    (void)workspace_bytes;
+    if (E < 0) return LSE_ERR_INVALID_ARG;
+    if (dtype != LSE_BF16 && dtype != LSE_F16) return LSE_ERR_UNSUPPORTED;
+    if (E == 0) return LSE_OK;
+    int rc = check_cache(H, H_kv, D, k_pool, v_pool, k_scale, v_scale, num_blocks, block_size);
+    if (rc) return rc;
+    if (!q || !o || !context_len) return LSE_ERR_INVALID_ARG;
+    if ((rc = check_table(block_table, bt_stride, bt_cols, E, block_size))) return rc;
+    if (!aligned(q, 16) || !aligned(o, 16) || q_stride_e % 8 || q_stride_h % 8 || o_stride_e % 8 || o_stride_h % 8 ||
+        !aligned(context_len, 4))
+        return LSE_ERR_ALIGNMENT;
+    int dev = 0;
+    if ((rc = host::current_device(&dev))) return rc;
+    kv8::AttnParams p{};
+    p.q = q;
+    p.q_st = q_stride_e;
+    p.q_sh = q_stride_h;
+    p.k_pool = k_pool;
+    p.v_pool = v_pool;
+    p.k_scale = k_scale;
+    p.v_scale = v_scale;
+    p.block_table = block_table;
+    p.bt_stride = bt_stride;
+    p.bt_cols = static_cast<int>(bt_cols);
+    p.context_len = context_len;
+    p.o = o;
+    p.o_st = o_stride_e;
+    p.o_sh = o_stride_h;
+    p.E = p.tokens = static_cast<int>(E);
+    p.H = static_cast<int>(H);
+    p.H_kv = static_cast<int>(H_kv);
+    p.block_size = static_cast<int>(block_size);
+    p.num_blocks = static_cast<int>(num_blocks);
+    p.scale_log2 = scale * 1.4426950408889634f;
+    return launch_attention(p, dtype, D, host::num_sms(dev), static_cast<cudaStream_t>(stream));
+}
+
+size_t lse_kv8_paged_attention_workspace(int64_t H, int64_t H_kv, int64_t D) {
+    (void)H;
+    (void)H_kv;
+    (void)D;
+    return 0;
+}
+
+int lse_kv8_paged_attention(const void *q, int dtype, int64_t tokens, int64_t H, int64_t D, int64_t q_stride_h,
+                            int64_t q_stride_m, const int8_t *k_pool, const int8_t *v_pool, const float *k_scale,
+                            const float *v_scale, int64_t num_blocks, int64_t block_size, int64_t H_kv,
+                            const int32_t *block_table, int64_t bt_stride, int64_t bt_cols, const int32_t *context_len,
+                            const int32_t *query_offset, const int32_t *q_start, const int32_t *q_len, int64_t E,
+                            float scale, void *o, int64_t o_stride_h, int64_t o_stride_m, void *workspace,
+                            size_t workspace_bytes, void *stream) {
+    (void)workspace;
+    (void)workspace_bytes;
+    if (E < 0 || tokens < 0) return LSE_ERR_INVALID_ARG;
+    if (dtype != LSE_BF16 && dtype != LSE_F16) return LSE_ERR_UNSUPPORTED;
+    if (E == 0 || tokens == 0) return LSE_OK;
+    int rc = check_cache(H, H_kv, D, k_pool, v_pool, k_scale, v_scale, num_blocks, block_size);
+    if (rc) return rc;
+    if (!q || !o || !context_len || !query_offset || !q_start || !q_len) return LSE_ERR_INVALID_ARG;
+    if ((rc = check_table(block_table, bt_stride, bt_cols, E, block_size))) return rc;
+    if (tokens > INT32_MAX / 2) return LSE_ERR_UNSUPPORTED;
+    if (!aligned(q, 16) || !aligned(o, 16) || q_stride_h % 8 || q_stride_m % 8 || o_stride_h % 8 || o_stride_m % 8 ||
+        !aligned(context_len, 4) || !aligned(query_offset, 4) || !aligned(q_start, 4) || !aligned(q_len, 4))
+        return LSE_ERR_ALIGNMENT;
+    int dev = 0;
+    if ((rc = host::current_device(&dev))) return rc;
+    kv8::AttnParams p{};
+    p.q = q;
+    p.q_st = q_stride_m;
+    p.q_sh = q_stride_h;
+    p.k_pool = k_pool;
+    p.v_pool = v_pool;
+    p.k_scale = k_scale;
+    p.v_scale = v_scale;
+    p.block_table = block_table;
+    p.bt_stride = bt_stride;
+    p.bt_cols = static_cast<int>(bt_cols);
+    p.context_len = context_len;
+    p.query_offset = query_offset;
+    p.q_start = q_start;
+    p.q_len = q_len;
+    p.o = o;
+    p.o_st = o_stride_m;
+    p.o_sh = o_stride_h;
+    p.E = static_cast<int>(E);
+    p.tokens = static_cast<int>(tokens);
+    p.H = static_cast<int>(H);
+    p.H_kv = static_cast<int>(H_kv);
+    p.block_size = static_cast<int>(block_size);
+    p.num_blocks = static_cast<int>(num_blocks);
+    p.scale_log2 = scale * 1.4426950408889634f;
+    return launch_attention(p, dtype, D, host::num_sms(dev), static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,56 @@
+// C-ABI entry point of the token log-probabilities (declared in include/lse_int8.h).
+#include <cuda_runtime.h>
+
+#include <climits>
+
+#include "../../include/lse_int8.h"
+#include "host.h"
+#include "logprobs.cuh"
+
+namespace lse {
+
+cudaError_t logprobs_device_status(int *status, bool reset) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_device_status, sizeof(int));
+    const int zero = LSE_OK;
+    if (e == cudaSuccess && reset) e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
+    return e;
+}
+
+}  // namespace lse
+
+using namespace lse;
+
+extern "C" int lse_token_logprobs(const void *logits, int dtype, int64_t M, int64_t V, int64_t ld, const int64_t *tokens,
+                                  int64_t top_k, float *logprob, float *entropy, float *top_logprobs, int64_t *top_ids,
+                                  void *stream) {
+    if (M < 0 || V <= 0 || top_k < 0 || top_k > V || ld < V) return LSE_ERR_INVALID_ARG;
+    if (dtype != LSE_BF16 && dtype != LSE_F16 && dtype != LSE_F32) return LSE_ERR_UNSUPPORTED;
+    if (M == 0) return LSE_OK;
+    if (!logits || !entropy || (tokens && !logprob) || (top_k && (!top_logprobs || !top_ids))) return LSE_ERR_INVALID_ARG;
+    if (M > INT32_MAX || V > INT32_MAX / 4 || top_k > LSE_LOGPROBS_MAX_TOP) return LSE_ERR_UNSUPPORTED;
+    const uintptr_t el = dtype == LSE_F32 ? 4 : 2;
+    auto off = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
+    if (off(logits, el) || off(tokens, 8) || off(logprob, 4) || off(entropy, 4) || off(top_logprobs, 4) || off(top_ids, 8))
+        return LSE_ERR_ALIGNMENT;
+    int dev = 0;
+    if (int rc = host::current_device(&dev)) return rc;
+    logprobs::Params p{};
+    p.x = logits;
+    p.ld = ld;
+    p.tokens = tokens;
+    p.logprob = logprob;
+    p.entropy = entropy;
+    p.top_logprob = top_logprobs;
+    p.top_id = top_ids;
+    p.M = static_cast<int>(M);
+    p.V = static_cast<int>(V);
+    p.k = static_cast<int>(top_k);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(M)), dim3(logprobs::THREADS), 0, static_cast<cudaStream_t>(stream));
+    const auto kernel = dtype == LSE_F32 ? logprobs::rows_kernel<float>
+                        : dtype == LSE_F16 ? logprobs::rows_kernel<__half> : logprobs::rows_kernel<__nv_bfloat16>;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? LSE_OK : host::cuda_error(e, "token_logprobs launch");
+}

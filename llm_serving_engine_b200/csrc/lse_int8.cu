@@ -15,6 +15,7 @@
 #include <mutex>
 
 #include "../../include/lse_int8.h"
+#include "host.h"
 #include "decode_attn.cuh"
 #include "paged_attn.cuh"
 #include "rope_kv.cuh"
@@ -900,6 +901,23 @@ extern "C" int lse_paged_attention(const void *q, int dtype, int64_t H, int64_t 
     return LSE_OK;
 }
 
+namespace lse {
+namespace host {
+
+int current_device(int *dev) { return lse::current_device(dev); }
+int num_sms(int dev) { return g_dev[dev].num_sms; }
+int cuda_error(cudaError_t e, const char *where) {
+    set_cuda_error(e, where);
+    return LSE_ERR_CUDA;
+}
+void launch_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&attr)[1], dim3 grid, dim3 block, size_t smem,
+                   cudaStream_t st) {
+    lse::launch_config(cfg, attr, grid, block, smem, st);
+}
+
+}  // namespace host
+}  // namespace lse
+
 extern "C" {
 
 int lse_set_wait_limit(int device, long long cycles) {
@@ -933,6 +951,12 @@ int lse_device_status(int device, int reset) {
     if (e == cudaSuccess && reset) {
         const int zero = LSE_OK;
         e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
+    }
+    // the other translation units' words
+    for (auto read : {kv8_device_status, logprobs_device_status}) {
+        int other = LSE_OK;
+        if (e == cudaSuccess) e = read(&other, reset != 0);
+        if (status == LSE_OK) status = other;
     }
     if (prev != device) cudaSetDevice(prev);
     if (e != cudaSuccess) { set_cuda_error(e, "lse_device_status"); return LSE_ERR_CUDA; }

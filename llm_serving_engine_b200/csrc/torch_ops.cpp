@@ -8,6 +8,10 @@
 //       (lse_int8_linear_packed_dt); x bf16 or fp16, y of x's dtype
 //   lse::gate_up_silu(Tensor x, Tensor w_packed, Tensor scale, int I, int K) -> Tensor
 //       silu(x @ Wg^T * sg) * (x @ Wu^T * su), [..., I] (lse_int8_gate_up_silu_packed_dt)
+//   lse::kv8_rope_append, lse::kv8_read, lse::kv8_decode_attention, lse::kv8_paged_attention
+//       the 8-bit paged K/V cache (lse_kv8_*); append writes the cache's four tensors
+//   lse::token_logprobs(Tensor logits, Tensor? tokens, int top_k)
+//       (logprob, entropy, top_logprobs, top_ids) of logits [..., V] (lse_token_logprobs)
 //
 // Errors come back as c10::Error (RuntimeError in Python) before any launch when an argument
 // is wrong, and with the library's status text when a launch is refused.  CUDA tensors only:
@@ -17,7 +21,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <map>
 #include <mutex>
+#include <utility>
 
 #include "../../include/lse_int8.h"
 
@@ -123,14 +129,256 @@ at::Tensor gate_up_silu(const at::Tensor &x, const at::Tensor &w_packed, const a
     return y;
 }
 
+// ---- the 8-bit paged K/V cache ------------------------------------------------------------
+struct Cache {
+    const at::Tensor &k, &v, &k_scale, &v_scale;
+    int64_t num_blocks() const { return k.size(0); }
+    int64_t H_kv() const { return k.size(1); }
+    int64_t block_size() const { return k.size(2); }
+    int64_t D() const { return k.size(3); }
+};
+
+void check_cuda(const at::Tensor &t, const at::Device &device, const char *what) {
+    TORCH_CHECK(t.is_cuda(), what, ": CUDA tensors only (no CPU fallback)");
+    TORCH_CHECK(t.device() == device, what, ": tensors on different devices");
+}
+
+void check_pool(const at::Tensor &pool, const at::Tensor &scale, const at::Device &device, const char *what) {
+    check_cuda(pool, device, what);
+    check_cuda(scale, device, what);
+    TORCH_CHECK(pool.scalar_type() == at::kChar && pool.dim() == 4 && pool.is_contiguous(), what,
+                ": pools must be contiguous int8 [num_blocks, H_kv, block_size, D]");
+    TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.dim() == 2 && scale.is_contiguous() &&
+                    scale.size(0) == pool.size(0) && scale.size(1) == pool.size(1),
+                what, ": scales must be contiguous float32 [num_blocks, H_kv]");
+}
+
+void check_cache(const Cache &c, const at::Device &device, const char *what) {
+    check_pool(c.k, c.k_scale, device, what);
+    check_pool(c.v, c.v_scale, device, what);
+    TORCH_CHECK(c.k.sizes() == c.v.sizes(), what, ": k and v pools of different shapes");
+}
+
+void check_i32(const at::Tensor &t, int64_t E, const at::Device &device, const char *what, const char *name) {
+    check_cuda(t, device, what);
+    TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == E && t.is_contiguous(), what, ": ", name,
+                " must be contiguous int32 [", E, "]");
+}
+
+void check_table(const at::Tensor &t, const at::Device &device, const char *what) {
+    check_cuda(t, device, what);
+    TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), what,
+                ": block_table must be int32 [E, n] with contiguous rows");
+}
+
+void check_launch(int rc, const char *name) {
+    TORCH_CHECK(rc == LSE_OK, name, ": ", lse_status_string(rc), rc == LSE_ERR_CUDA ? " " : "",
+                rc == LSE_ERR_CUDA ? lse_last_cuda_error() : "");
+}
+
+// A 3-D tensor the kernels can read with 16-byte loads (itself, or a contiguous copy).
+at::Tensor rows16(const at::Tensor &x) {
+    const bool ok = x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+at::Tensor kv8_rope_append(const at::Tensor &qkv, int64_t n_heads, const at::Tensor &k, const at::Tensor &v,
+                           const at::Tensor &k_scale, const at::Tensor &v_scale, const at::Tensor &block_table,
+                           const at::Tensor &query_offset, const at::Tensor &q_start, const at::Tensor &q_len,
+                           const c10::optional<at::Tensor> &cos, const c10::optional<at::Tensor> &sin, bool interleaved) {
+    const char *what = "lse::kv8_rope_append";
+    const Cache c{k, v, k_scale, v_scale};
+    const at::Device dev = qkv.device();
+    check_cuda(qkv, dev, what);
+    check_cache(c, dev, what);
+    check_table(block_table, dev, what);
+    const int64_t E = block_table.size(0), D = c.D(), M = qkv.dim() == 2 ? qkv.size(0) : -1;
+    const int dt = dtype_code(qkv);
+    TORCH_CHECK(n_heads > 0 && qkv.dim() == 2 && qkv.size(1) == (n_heads + 2 * c.H_kv()) * D, what,
+                ": qkv must be [M, (H + 2 H_kv) * D]");
+    check_i32(query_offset, E, dev, what, "query_offset");
+    check_i32(q_start, E, dev, what, "q_start");
+    check_i32(q_len, E, dev, what, "q_len");
+    const bool turn = cos.has_value() && cos->defined();
+    TORCH_CHECK(turn == (sin.has_value() && sin->defined()), what, ": cos and sin come together");
+    int64_t R = 0, ld_cs = 0;
+    int cs = LSE_F32;
+    if (turn) {
+        check_cuda(*cos, dev, what);
+        check_cuda(*sin, dev, what);
+        TORCH_CHECK(cos->dim() == 2 && cos->size(0) == M && cos->size(1) <= D && cos->size(1) % 2 == 0 &&
+                        cos->sizes() == sin->sizes() && cos->strides() == sin->strides() &&
+                        (cos->size(1) <= 1 || cos->stride(1) == 1) && cos->scalar_type() == sin->scalar_type(),
+                    what, ": cos and sin must be [M, R], R even and at most D, with equal, row-contiguous strides");
+        TORCH_CHECK(cos->scalar_type() == at::kFloat || cos->scalar_type() == at::kBFloat16 || cos->scalar_type() == at::kHalf,
+                    what, ": cos and sin must be float32, bfloat16 or float16");
+        cs = cos->scalar_type() == at::kFloat ? LSE_F32 : dtype_code(*cos);
+        R = cos->size(1);
+        ld_cs = M > 1 ? cos->stride(0) : R;
+    }
+    c10::cuda::CUDAGuard guard(dev);
+    init_device(dev.index());
+    at::Tensor q = at::empty({n_heads, M, D}, qkv.options());
+    if (M == 0) return q;
+    at::Tensor x = qkv;
+    if (x.stride(1) != 1 || (M > 1 && (x.stride(0) % 8 || x.stride(0) < x.size(1))) || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16)
+        x = x.clone(at::MemoryFormat::Contiguous);
+    check_launch(lse_kv8_rope_append(x.data_ptr(), dt, M, M > 1 ? x.stride(0) : x.size(1), n_heads, c.H_kv(), D,
+                                     R ? cos->data_ptr() : nullptr, R ? sin->data_ptr() : nullptr, ld_cs, cs, R, interleaved,
+                                     q.data_ptr(), k.data_ptr<int8_t>(), v.data_ptr<int8_t>(), k_scale.data_ptr<float>(),
+                                     v_scale.data_ptr<float>(), c.num_blocks(), c.block_size(), block_table.data_ptr<int>(),
+                                     block_table.stride(0), block_table.size(1), query_offset.data_ptr<int>(),
+                                     q_start.data_ptr<int>(), q_len.data_ptr<int>(), E, at::cuda::getCurrentCUDAStream(dev.index()).stream()),
+                 "lse_kv8_rope_append");
+    return q;
+}
+
+std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_scale,
+                                            const at::Tensor &v_scale, const at::Tensor &block_ids, at::ScalarType dtype) {
+    const char *what = "lse::kv8_read";
+    const Cache c{k, v, k_scale, v_scale};
+    const at::Device dev = k.device();
+    check_cuda(k, dev, what);
+    check_cache(c, dev, what);
+    check_cuda(block_ids, dev, what);
+    TORCH_CHECK(block_ids.scalar_type() == at::kLong && block_ids.dim() == 1 && block_ids.is_contiguous(), what,
+                ": block_ids must be contiguous int64 [n]");
+    TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, what, ": values are bfloat16 or float16, not ", dtype);
+    c10::cuda::CUDAGuard guard(dev);
+    init_device(dev.index());
+    const int64_t n = block_ids.size(0);
+    const auto options = k.options().dtype(dtype);
+    at::Tensor out[2] = {at::empty({n, c.H_kv(), c.block_size(), c.D()}, options),
+                         at::empty({n, c.H_kv(), c.block_size(), c.D()}, options)};
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const int dt = dtype == at::kHalf ? LSE_F16 : LSE_BF16;
+    for (int i = 0; i < 2; ++i)
+        check_launch(lse_kv8_read((i ? v : k).data_ptr<int8_t>(), (i ? v_scale : k_scale).data_ptr<float>(), c.num_blocks(),
+                                  c.block_size(), c.H_kv(), c.D(), block_ids.data_ptr<int64_t>(), n, out[i].data_ptr(), dt, st),
+                     "lse_kv8_read");
+    return {out[0], out[1]};
+}
+
+at::Tensor kv8_decode_attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_scale,
+                                const at::Tensor &v_scale, const at::Tensor &block_table, const at::Tensor &context_len,
+                                double scale) {
+    const char *what = "lse::kv8_decode_attention";
+    const Cache c{k, v, k_scale, v_scale};
+    const at::Device dev = q.device();
+    check_cuda(q, dev, what);
+    check_cache(c, dev, what);
+    check_table(block_table, dev, what);
+    const int dt = dtype_code(q);
+    const int64_t E = block_table.size(0);
+    TORCH_CHECK(q.dim() == 3 && q.size(0) == E && q.size(2) == c.D(), what, ": q must be [E, H, D] with the cache's D");
+    check_i32(context_len, E, dev, what, "context_len");
+    c10::cuda::CUDAGuard guard(dev);
+    init_device(dev.index());
+    at::Tensor o = at::empty({E, q.size(1), c.D()}, q.options());
+    if (E == 0 || q.size(1) == 0) return o;
+    const at::Tensor x = rows16(q);
+    check_launch(lse_kv8_decode_attention(x.data_ptr(), dt, E, q.size(1), c.D(), x.stride(0), x.stride(1), k.data_ptr<int8_t>(),
+                                          v.data_ptr<int8_t>(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
+                                          c.num_blocks(), c.block_size(), c.H_kv(), block_table.data_ptr<int>(),
+                                          block_table.stride(0), block_table.size(1), context_len.data_ptr<int>(),
+                                          static_cast<float>(scale), o.data_ptr(), o.stride(0), o.stride(1), nullptr, 0,
+                                          at::cuda::getCurrentCUDAStream(dev.index()).stream()),
+                 "lse_kv8_decode_attention");
+    return o;
+}
+
+at::Tensor kv8_paged_attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_scale,
+                               const at::Tensor &v_scale, const at::Tensor &block_table, const at::Tensor &context_len,
+                               const at::Tensor &query_offset, const at::Tensor &q_start, const at::Tensor &q_len,
+                               double scale) {
+    const char *what = "lse::kv8_paged_attention";
+    const Cache c{k, v, k_scale, v_scale};
+    const at::Device dev = q.device();
+    check_cuda(q, dev, what);
+    check_cache(c, dev, what);
+    check_table(block_table, dev, what);
+    const int dt = dtype_code(q);
+    const int64_t E = block_table.size(0);
+    TORCH_CHECK(q.dim() == 3 && q.size(2) == c.D(), what, ": q must be [H, tokens, D] with the cache's D");
+    check_i32(context_len, E, dev, what, "context_len");
+    check_i32(query_offset, E, dev, what, "query_offset");
+    check_i32(q_start, E, dev, what, "q_start");
+    check_i32(q_len, E, dev, what, "q_len");
+    c10::cuda::CUDAGuard guard(dev);
+    init_device(dev.index());
+    at::Tensor o = at::empty({q.size(0), q.size(1), c.D()}, q.options());
+    if (E == 0 || q.size(0) == 0 || q.size(1) == 0) return o;
+    const at::Tensor x = rows16(q);
+    check_launch(lse_kv8_paged_attention(x.data_ptr(), dt, q.size(1), q.size(0), c.D(), x.stride(0), x.stride(1),
+                                         k.data_ptr<int8_t>(), v.data_ptr<int8_t>(), k_scale.data_ptr<float>(),
+                                         v_scale.data_ptr<float>(), c.num_blocks(), c.block_size(), c.H_kv(),
+                                         block_table.data_ptr<int>(), block_table.stride(0), block_table.size(1),
+                                         context_len.data_ptr<int>(), query_offset.data_ptr<int>(), q_start.data_ptr<int>(),
+                                         q_len.data_ptr<int>(), E, static_cast<float>(scale), o.data_ptr(), o.stride(0),
+                                         o.stride(1), nullptr, 0, at::cuda::getCurrentCUDAStream(dev.index()).stream()),
+                 "lse_kv8_paged_attention");
+    return o;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(const at::Tensor &logits,
+                                                                          const c10::optional<at::Tensor> &tokens,
+                                                                          int64_t top_k) {
+    const char *what = "lse::token_logprobs";
+    const at::Device dev = logits.device();
+    check_cuda(logits, dev, what);
+    TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) > 0, what, ": logits must be [..., V]");
+    const int dt = logits.scalar_type() == at::kFloat ? LSE_F32 : dtype_code(logits);
+    const int64_t V = logits.size(-1);
+    TORCH_CHECK(top_k >= 0 && top_k <= std::min<int64_t>(V, LSE_LOGPROBS_MAX_TOP), what, ": top_k must be 0 .. min(V, ",
+                LSE_LOGPROBS_MAX_TOP, "), got ", top_k);
+    const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+    const bool given = tokens.has_value() && tokens->defined();
+    if (given) {
+        check_cuda(*tokens, dev, what);
+        TORCH_CHECK(tokens->scalar_type() == at::kLong && tokens->sizes() == lead, what, ": tokens must be int64 of logits' leading shape");
+    }
+    c10::cuda::CUDAGuard guard(dev);
+    init_device(dev.index());
+    at::Tensor x = logits.dim() == 2 ? logits : logits.reshape({-1, V});
+    const int64_t M = x.size(0);
+    if (x.stride(1) != 1 || (M > 1 && x.stride(0) < V)) x = x.clone(at::MemoryFormat::Contiguous);
+    const at::Tensor t = given ? tokens->contiguous() : at::Tensor();
+    const auto f32 = logits.options().dtype(at::kFloat);
+    std::vector<int64_t> shape(lead.begin(), lead.end());
+    at::Tensor logprob = given ? at::empty(shape, f32) : at::empty({0}, f32), entropy = at::empty(shape, f32);
+    shape.push_back(top_k);
+    at::Tensor top = at::empty(shape, f32), ids = at::empty(shape, logits.options().dtype(at::kLong));
+    if (M == 0) return {logprob, entropy, top, ids};
+    check_launch(lse_token_logprobs(x.data_ptr(), dt, M, V, M > 1 ? x.stride(0) : V, given ? t.data_ptr<int64_t>() : nullptr,
+                                    top_k, given ? logprob.data_ptr<float>() : nullptr, entropy.data_ptr<float>(),
+                                    top.data_ptr<float>(), ids.data_ptr<int64_t>(), at::cuda::getCurrentCUDAStream(dev.index()).stream()),
+                 "lse_token_logprobs");
+    return {logprob, entropy, top, ids};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(lse, m) {
     m.def("int8_linear(Tensor x, Tensor w_packed, Tensor scale, int N, int K, Tensor? residual=None, int algo=0) -> Tensor");
     m.def("gate_up_silu(Tensor x, Tensor w_packed, Tensor scale, int I, int K) -> Tensor");
+    m.def("kv8_rope_append(Tensor qkv, int n_heads, Tensor(a!) k, Tensor(b!) v, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+          "Tensor block_table, Tensor query_offset, Tensor q_start, Tensor q_len, Tensor? cos=None, Tensor? sin=None, "
+          "bool interleaved=False) -> Tensor");
+    m.def("kv8_read(Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor block_ids, ScalarType dtype) -> (Tensor, Tensor)");
+    m.def("kv8_decode_attention(Tensor q, Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor block_table, "
+          "Tensor context_len, float scale) -> Tensor");
+    m.def("kv8_paged_attention(Tensor q, Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor block_table, "
+          "Tensor context_len, Tensor query_offset, Tensor q_start, Tensor q_len, float scale) -> Tensor");
+    m.def("token_logprobs(Tensor logits, Tensor? tokens, int top_k) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(lse, CUDA, m) {
     m.impl("int8_linear", &int8_linear);
     m.impl("gate_up_silu", &gate_up_silu);
+    m.impl("kv8_rope_append", &kv8_rope_append);
+    m.impl("kv8_read", &kv8_read);
+    m.impl("kv8_decode_attention", &kv8_decode_attention);
+    m.impl("kv8_paged_attention", &kv8_paged_attention);
+    m.impl("token_logprobs", &token_logprobs);
 }

@@ -19,6 +19,7 @@ any stream, inside a capture or not, and nothing persists between calls.
 from __future__ import annotations
 
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -41,6 +42,8 @@ __all__ = [
     "rope_kv_write",
     "rms_norm", "rms_norm_proj",
     "pool_slot_offsets",
+    "Kv8Cache", "kv8_cache", "kv8_rope_append", "kv8_read", "kv8_decode_attention", "kv8_paged_attention",
+    "TokenLogprobs", "token_logprobs", "LOGPROBS_MAX_TOP",
     "linear_workspace",
     "device_status",
     "ALGO_AUTO",
@@ -521,6 +524,95 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         stream.cuda_stream)
     _lib.check(rc, "lse_paged_attention")
     return out
+
+
+class Kv8Cache(NamedTuple):
+    """One layer's paged K/V cache in 8 bits: int8 codes [num_blocks, H_kv, block_size, D] and one
+    fp32 scale per page and KV head [num_blocks, H_kv], value = code * scale."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def kv8_cache(num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int, device=None) -> Kv8Cache:
+    """An empty (zero) 8-bit cache; about half the bytes of a bf16 pool of the same positions."""
+    pool = dict(size=(num_blocks, n_kv_heads, block_size, head_dim), dtype=torch.int8, device=device or "cuda")
+    scale = dict(size=(num_blocks, n_kv_heads), dtype=torch.float32, device=device or "cuda")
+    return Kv8Cache(torch.zeros(**pool), torch.zeros(**pool), torch.zeros(**scale), torch.zeros(**scale))
+
+
+def _need_cuda(t: torch.Tensor, what: str):
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} runs on CUDA only (no CPU fallback)")
+    return torch.ops.lse if _torch_ops_loaded else torch_ops()
+
+
+def kv8_rope_append(qkv: torch.Tensor, n_heads: int, cache: Kv8Cache, block_table: torch.Tensor,
+                    query_offset: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
+                    cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+                    interleaved: bool = False) -> torch.Tensor:
+    """`rope_kv_write` for an 8-bit cache: q and k of the fused QKV output rotated, k and v
+    quantised into the entries' pages, q returned as (n_heads, tokens, head_dim), in one launch.
+
+    qkv: bf16 or fp16 [M, (H + 2 H_kv) * D]; row q_start[e] + i is position query_offset[e] + i of
+    entry e (i < q_len[e]), stored in page block_table[e, position // block_size] (all int32).
+    cos / sin: [M, R] fp32, bf16 or fp16, the first R dims of each head rotate (None: no
+    rotation), in halves (dims d and d + R/2) or `interleaved` pairs (2i and 2i + 1), the tables
+    holding one value per dim.  A page's scale is max |x| / 127 over all it holds: a larger
+    value that arrives later rescales the page's earlier codes.  Pages of two entries of one call
+    must differ; a page outside the pool is skipped and reported by `device_status`.
+    """
+    return _need_cuda(qkv, "kv8_rope_append").kv8_rope_append(qkv, n_heads, *cache, block_table, query_offset, q_start,
+                                                              q_len, cos, sin, interleaved)
+
+
+def kv8_read(cache: Kv8Cache, block_ids: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of the pages `block_ids` (int64 [n]): k and v [n, H_kv, block_size, D] in bf16
+    or fp16, code * scale rounded once."""
+    return _need_cuda(block_ids, "kv8_read").kv8_read(*cache, block_ids, dtype)
+
+
+def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Tensor, context_len: torch.Tensor,
+                         scale: float | None = None) -> torch.Tensor:
+    """`paged_decode_attention` over an 8-bit cache: q bf16 or fp16 [E, H, D], one query token per
+    entry attending to its first context_len[e] positions (int32, at most the block table's width
+    times block_size: a longer one is cut and reported by `device_status`); [E, H, D] of q's dtype.
+    The launch is the same for every batch and context length."""
+    return _need_cuda(q, "kv8_decode_attention").kv8_decode_attention(
+        q, *cache, block_table, context_len, q.shape[-1] ** -0.5 if scale is None else scale)
+
+
+def kv8_paged_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Tensor, context_len: torch.Tensor,
+                        query_offset: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
+                        scale: float | None = None) -> torch.Tensor:
+    """`paged_attention` over an 8-bit cache: q bf16 or fp16 (H, tokens, D), entry e's rows
+    q_start[e] .. + q_len[e] - 1 at positions query_offset[e] + i attending causally to the positions
+    below context_len[e]; o like q.  Rows of no entry are left unwritten."""
+    return _need_cuda(q, "kv8_paged_attention").kv8_paged_attention(
+        q, *cache, block_table, context_len, query_offset, q_start, q_len, q.shape[-1] ** -0.5 if scale is None else scale)
+
+
+LOGPROBS_MAX_TOP = _lib.LOGPROBS_MAX_TOP
+
+
+class TokenLogprobs(NamedTuple):
+    """What `token_logprobs` returns: fp32 log-probability of the given tokens (empty without
+    tokens), fp32 entropy, and the top alternatives' fp32 log-probabilities and int64 ids."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_ids: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0) -> TokenLogprobs:
+    """Log-probabilities of `tokens` (int64 [...]) under `logits` ([..., V] bf16, fp16 or fp32), the
+    entropy of each row in nats, and the `top_k` likeliest tokens (0 .. min(V, LOGPROBS_MAX_TOP),
+    equal logits by index, lowest first), fp32 throughout.  -inf logits have probability 0; a row
+    without any other has log-probabilities -inf and entropy 0; a NaN or +inf makes its row NaN."""
+    return TokenLogprobs(*_need_cuda(logits, "token_logprobs").token_logprobs(logits, tokens, top_k))
 
 
 def set_wait_limit(cycles: int, device: int | torch.device | None = None) -> None:

@@ -1,0 +1,110 @@
+"""CPU oracle of the 8-bit paged K/V cache and the token log-probabilities (test infrastructure
+only, float64): the definitions in include/lse_int8.h written out directly."""
+
+from __future__ import annotations
+
+import numpy as np
+
+__all__ = ["ref_rotate", "ref_append", "ref_attention", "ref_logprobs"]
+
+
+def ref_rotate(x: np.ndarray, cos: np.ndarray, sin: np.ndarray, interleaved: bool) -> np.ndarray:
+    """x [M, heads, D] with the first R = cos.shape[1] dims rotated (cos, sin [M, R])."""
+    out = x.astype(np.float64).copy()
+    R = cos.shape[1]
+    for d in range(R):
+        if interleaved:
+            other, sign = (d + 1, -1.0) if d % 2 == 0 else (d - 1, 1.0)
+        else:
+            other, sign = (d + R // 2, -1.0) if d < R // 2 else (d - R // 2, 1.0)
+        out[..., d] = x[..., d] * cos[:, None, d] + sign * x[..., other] * sin[:, None, d]
+    return out
+
+
+def ref_append(codes, scale, new, table, offset, start, length, bs):
+    """Appends new [M, H_kv, D] to a pool (codes [nb, H_kv, bs, D], scale [nb, H_kv]); returns the new
+    pool and, for each new row and head, its unrounded code (x / s), and the same for earlier codes."""
+    codes, scale = codes.astype(np.float64).copy(), scale.astype(np.float64).copy()
+    exact = codes.copy()
+    for e in range(len(length)):
+        p = int(offset[e])
+        end = p + int(length[e])
+        while p < end:
+            page, stop = p // bs, min(end, (p // bs + 1) * bs)
+            b, old = int(table[e, page]), p - (p // bs) * bs
+            row = int(start[e]) + p - int(offset[e])
+            for h in range(codes.shape[1]):
+                x = new[row:row + stop - p, h]
+                before = scale[b, h] if old else 0.0
+                if not np.all(np.isfinite(x)) or np.isnan(before):
+                    scale[b, h] = np.nan
+                    codes[b, h, old:old + stop - p] = exact[b, h, old:old + stop - p] = 0.0
+                    continue
+                s = max(before, np.abs(x).max() / 127.0)
+                if old and s > before:
+                    exact[b, h, :old] = codes[b, h, :old] * (before / s)
+                    codes[b, h, :old] = np.rint(exact[b, h, :old])
+                exact[b, h, old:old + stop - p] = x / s if s > 0 else 0.0
+                codes[b, h, old:old + stop - p] = np.clip(np.rint(exact[b, h, old:old + stop - p]), -127, 127)
+                scale[b, h] = s
+            p = stop
+    return codes, scale, exact
+
+
+def ref_attention(q, k, v, k_scale, v_scale, table, context, offset=None, start=None, length=None, scale=None):
+    """q [tokens, H, D] over pools [nb, H_kv, bs, D]; returns o and sum_p w_p |v_p| (the size that
+    rounding errors of the weights act on).  Without offset: one query per entry at its end."""
+    tokens, H, D = q.shape
+    H_kv, bs = k.shape[1], k.shape[2]
+    scale = D ** -0.5 if scale is None else scale
+    o, size = np.zeros((tokens, H, D)), np.zeros((tokens, H, D))
+    written = np.zeros(tokens, dtype=bool)
+    for e in range(len(context)):
+        n = 1 if offset is None else int(length[e])
+        for i in range(n):
+            t = e if offset is None else int(start[e]) + i
+            limit = int(context[e]) if offset is None else min(int(context[e]), int(offset[e]) + i + 1)
+            written[t] = True
+            if limit <= 0:
+                continue
+            pos = np.arange(limit)
+            page = table[e, pos // bs]
+            ok = (page >= 0) & (page < k.shape[0])
+            page, slot = page[ok], (pos % bs)[ok]
+            if not len(page):
+                continue
+            for h in range(H):
+                g = h // (H // H_kv)
+                kk = k[page, g, slot].astype(np.float64) * k_scale[page, g, None].astype(np.float64)
+                vv = v[page, g, slot].astype(np.float64) * v_scale[page, g, None].astype(np.float64)
+                s = kk @ q[t, h].astype(np.float64) * scale
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                o[t, h], size[t, h] = w @ vv, w @ np.abs(vv)
+    return o, size, written
+
+
+def ref_logprobs(x, tokens, k):
+    """(logprob, entropy, top log-probabilities, top ids) of rows of logits [M, V] in float64."""
+    M, V = x.shape
+    lp, ent = np.full(M, np.nan), np.full(M, np.nan)
+    top, ids = np.full((M, k), np.nan), np.zeros((M, k), dtype=np.int64)
+    for m in range(M):
+        r = x[m].astype(np.float64)
+        order = np.where(np.isnan(r), np.inf, r)
+        # NaN above +inf, then by value, then by index
+        ids[m] = np.lexsort((np.arange(V), -order, ~np.isnan(r)))[:k]
+        if np.isnan(r).any() or np.isposinf(r).any():
+            continue
+        if np.isneginf(r).all():
+            all_lp, ent[m] = r, 0.0
+        else:
+            d = r - r.max()
+            z = np.exp(d).sum()
+            all_lp = d - np.log(z)
+            live = np.exp(d) > 0
+            ent[m] = np.log(z) - (d[live] * np.exp(d[live])).sum() / z
+        top[m] = all_lp[ids[m]]
+        if tokens is not None and 0 <= tokens[m] < V:
+            lp[m] = all_lp[tokens[m]]
+    return lp, ent, top, ids
