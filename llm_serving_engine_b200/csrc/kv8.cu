@@ -9,6 +9,7 @@
 #include "host.h"
 #include "kv8_append.cuh"
 #include "kv8_attn.cuh"
+#include "kv8_decode.cuh"
 
 namespace lse {
 
@@ -30,7 +31,8 @@ int check_cache(int64_t H, int64_t H_kv, int64_t D, const void *k_pool, const vo
     if (!k_pool || !v_pool || !k_scale || !v_scale) return LSE_ERR_INVALID_ARG;
     const int64_t G = H / H_kv;
     if ((D != 64 && D != 128) || (G != 1 && G != 2 && G != 4 && G != 8)) return LSE_ERR_UNSUPPORTED;
-    if (H > 65535 || block_size > 65536 || num_blocks > INT32_MAX / 2 || num_blocks * block_size > INT32_MAX / 2)
+    if (H > 65535 || block_size > 65536 || num_blocks > INT32_MAX / 2 || num_blocks * block_size > INT32_MAX / 2 ||
+        num_blocks * block_size / 8 * H_kv > INT32_MAX)
         return LSE_ERR_UNSUPPORTED;
     if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
         return LSE_ERR_ALIGNMENT;
@@ -108,6 +110,33 @@ int launch_rows(const kv8::AttnParams &p, int sms, cudaStream_t st) {
     return finish(cudaLaunchKernelEx(&cfg, kv8::attn_rows_kernel<D, T>, p), "kv8 attention launch");
 }
 
+// Resident CTAs per SM of the decode kernel (its launch bounds) and so the launch's grid.
+constexpr int kDecodePerSm = 3;
+
+size_t decode_counter_bytes(int sms) { return (static_cast<size_t>(kDecodePerSm) * sms * sizeof(int) + 255) / 256 * 256; }
+
+template <int D, int G, typename T>
+int launch_decode(const kv8::AttnParams &p, const kv8::DecodeWork &w, int sms, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    const bool paged8 = p.block_size % 8 == 0;
+    const int grid = kDecodePerSm * sms;
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(grid)), dim3(kv8::DEC_THREADS), 0, st);
+    return finish(paged8 ? cudaLaunchKernelEx(&cfg, kv8::decode_kernel<D, G, T, true>, p, w)
+                         : cudaLaunchKernelEx(&cfg, kv8::decode_kernel<D, G, T, false>, p, w),
+                  "kv8_decode_attention launch");
+}
+
+template <int D, typename T>
+int launch_decode_g(int64_t G, const kv8::AttnParams &p, const kv8::DecodeWork &w, int sms, cudaStream_t st) {
+    switch (G) {
+        case 1: return launch_decode<D, 1, T>(p, w, sms, st);
+        case 2: return launch_decode<D, 2, T>(p, w, sms, st);
+        case 4: return launch_decode<D, 4, T>(p, w, sms, st);
+        default: return launch_decode<D, 8, T>(p, w, sms, st);
+    }
+}
+
 int launch_attention(const kv8::AttnParams &p, int dtype, int64_t D, int sms, cudaStream_t st) {
     if (dtype == LSE_F16) return D == 128 ? launch_rows<128, __half>(p, sms, st) : launch_rows<64, __half>(p, sms, st);
     return D == 128 ? launch_rows<128, __nv_bfloat16>(p, sms, st) : launch_rows<64, __nv_bfloat16>(p, sms, st);
@@ -175,10 +204,10 @@ int lse_kv8_read(const int8_t *pool, const float *scale, int64_t num_blocks, int
 }
 
 size_t lse_kv8_decode_attention_workspace(int64_t H, int64_t H_kv, int64_t D) {
-    (void)H;
-    (void)H_kv;
-    (void)D;
-    return 0;
+    int dev = 0;
+    if (H <= 0 || H_kv <= 0 || D <= 0 || H % H_kv || host::current_device(&dev)) return 0;
+    const int sms = host::num_sms(dev);
+    return decode_counter_bytes(sms) + 2ull * kDecodePerSm * sms * (H / H_kv) * (D + 2) * sizeof(float);
 }
 
 int lse_kv8_decode_attention(const void *q, int dtype, int64_t E, int64_t H, int64_t D, int64_t q_stride_e,
@@ -187,8 +216,6 @@ int lse_kv8_decode_attention(const void *q, int dtype, int64_t E, int64_t H, int
                              const int32_t *block_table, int64_t bt_stride, int64_t bt_cols, const int32_t *context_len,
                              float scale, void *o, int64_t o_stride_e, int64_t o_stride_h, void *workspace,
                              size_t workspace_bytes, void *stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     if (E < 0) return LSE_ERR_INVALID_ARG;
     if (dtype != LSE_BF16 && dtype != LSE_F16) return LSE_ERR_UNSUPPORTED;
     if (E == 0) return LSE_OK;
@@ -222,7 +249,18 @@ int lse_kv8_decode_attention(const void *q, int dtype, int64_t E, int64_t H, int
     p.block_size = static_cast<int>(block_size);
     p.num_blocks = static_cast<int>(num_blocks);
     p.scale_log2 = scale * 1.4426950408889634f;
-    return launch_attention(p, dtype, D, host::num_sms(dev), static_cast<cudaStream_t>(stream));
+    if (!workspace || workspace_bytes < lse_kv8_decode_attention_workspace(H, H_kv, D)) return LSE_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return LSE_ERR_ALIGNMENT;
+    const int sms = host::num_sms(dev);
+    const int64_t G = H / H_kv;
+    kv8::DecodeWork w{};
+    w.counters = static_cast<int *>(workspace);
+    w.acc = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + decode_counter_bytes(sms));
+    w.ml = w.acc + 2ll * kDecodePerSm * sms * G * D;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == LSE_F16)
+        return D == 128 ? launch_decode_g<128, __half>(G, p, w, sms, st) : launch_decode_g<64, __half>(G, p, w, sms, st);
+    return D == 128 ? launch_decode_g<128, __nv_bfloat16>(G, p, w, sms, st) : launch_decode_g<64, __nv_bfloat16>(G, p, w, sms, st);
 }
 
 size_t lse_kv8_paged_attention_workspace(int64_t H, int64_t H_kv, int64_t D) {

@@ -1,0 +1,611 @@
+// Decode attention (one query token per sequence) over the 8-bit paged K/V cache:
+//
+//   o[e, h, :] = sum_p w_p v_scale[b_p] v_code[p, :] / sum_p w_p,
+//   w_p = 2^(t_p),  t_p = scale log2(e) k_scale[b_p] (q[e, h, :] . k_code[p, :])
+//
+// A stream over the cache: 2 D bytes a position and KV head, shared by the G = H / H_kv query
+// heads.  What the kernel is shaped by:
+//   * The codes go from global memory straight into the registers of the warp MMA's row operand
+//     (m16n8k16): S^T = K Q^T has 16 positions as rows and the query heads as its 8 columns, and
+//     O^T += V^T P^T has 16 dims as rows.  The order of a contraction's index is free, so a thread's
+//     operand is made of 16-byte runs of a row: K row r0 (and r0 + 8), chunks q4 and q4 + 4; V rows
+//     2 q4, 2 q4 + 1 (+ 8), chunk r0 (r0 = lane / 4, q4 = lane % 4).  No shared memory, no barrier
+//     in the loop; the next tile's loads are in flight under the current one's arithmetic.
+//   * int8 -> fp16 is exact: one byte permute puts a biased code under the exponent of 1024, one
+//     subtraction takes the bias off.  q is fp16 after an exact power-of-two scaling per head (bf16)
+//     or as it is; scores are fp32 sums of exact products.
+//   * The page's K scale multiplies the scores, its V scale the weights.  P is rounded to fp16
+//     relative to M >= max_p (t_p + log2 v_scale) - 6, the largest thing that enters the sum over V,
+//     so pages of very different sizes keep 11 bits; the sum of weights stays fp32.  M (and with
+//     it the accumulators) moves only when something exceeds it by 2^6: one vote a tile.
+//   * The work is cut by positions, not by sequences: the pairs (sequence, KV head) laid end to
+//     end in chunks of CHUNK positions are dealt to the CTAs in equal runs, from context_len on
+//     the device, so a ragged batch and a single long sequence fill the GPU alike, and the launch
+//     is the same for every batch.  A pair that several CTAs share is joined by the CTA that
+//     arrives last, in the order of the positions (deterministic); none waits for another.
+#pragma once
+
+#include "common.cuh"
+#include "kv8_attn.cuh"
+
+namespace lse {
+namespace kv8 {
+
+constexpr int DEC_WARPS = 4;
+constexpr int DEC_THREADS = DEC_WARPS * 32;
+constexpr int DEC_MAX_SPLITS = 64;  // CTAs that share a pair, at most (+ 1 by rounding)
+
+// A tile is what one warp takes at a time; a chunk one tile for each warp.
+template <int D>
+constexpr int DEC_TILE = 16 * (128 / D);
+template <int D>
+constexpr int DEC_CHUNK = DEC_WARPS * DEC_TILE<D>;
+
+struct DecodeWork {
+    int *counters;  // [grid] arrivals at the pair that starts last in a CTA, zero between launches
+    float *acc;     // [2 * grid][G * D] partial sums: of the pair that a CTA continues, of the one it begins
+    float *ml;      // [2 * grid][G][2] their M and sum of weights
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {  // 2^x, relative error 2^-22; 2^-inf = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 ld_stream16(const int8_t *p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint2 ld_stream8(const int8_t *p) {
+    uint2 r;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movm_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Bytes 0 and 1 (or 2 and 3) of a word of biased codes (code ^ 0x80) as two halves, exact:
+// 0x64uu is 1024 + u, and 1024 + u - 1152 the code.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t u) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t u) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(0x64806480u));
+    return r;
+}
+
+// PAGED8: block_size is a multiple of 8, so that 8 consecutive positions share a page and its scales;
+// otherwise every position looks its page up for itself.
+template <int D, int G, typename T, bool PAGED8>
+__global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams p, const DecodeWork w) {
+    constexpr int U = 128 / D;          // 16-position MMA rows of a tile
+    constexpr int TILE = DEC_TILE<D>, CHUNK = DEC_CHUNK<D>;
+    constexpr int KC = D / 64;          // 16-byte chunks of a K row per thread
+    constexpr int VW = D / 32;          // words of a V row per thread
+    constexpr int MT = D / 16;          // 16-dim row tiles of O^T
+    constexpr float M_NONE = -1e30f;    // below every score; finite, so that 2^(-inf - M) is 0
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r0 = lane >> 2, q4 = lane & 3;
+    const int64_t table_positions = static_cast<int64_t>(p.bt_cols) * p.block_size;
+
+    __shared__ float s_acc[DEC_WARPS][G][D + 4];
+    __shared__ float s_ml[DEC_WARPS][G][2];
+    __shared__ float s_w[DEC_MAX_SPLITS + 2][G], s_l[G];
+    __shared__ int s_scan[DEC_WARPS], s_max[DEC_WARPS];
+    __shared__ int s_at[3];
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the cache and the lengths come from earlier kernels
+
+    auto context = [&](int e) {  // positions of entry e, cut to its table
+        const int c = __ldcg(p.context_len + e);
+        return static_cast<int>(min(static_cast<int64_t>(max(c, 0)), table_positions));
+    };
+    auto chunks_of = [](int ctx) { return max(1, (ctx + CHUNK - 1) / CHUNK); };
+
+    // ---- the run of chunks of this CTA -------------------------------------------------------
+    // Every CTA adds up all lengths (E is small); an entry has chunks_of(context) * H_kv chunks.
+    int64_t total = 0;
+    int longest = 0;
+    for (int e0 = 0; e0 < p.E; e0 += DEC_THREADS) {
+        const int e = e0 + threadIdx.x;
+        int n = 0;
+        if (e < p.E) {
+            n = chunks_of(context(e));
+            if (blockIdx.x == 0 && __ldcg(p.context_len + e) > table_positions) report_status(LSE_ERR_INVALID_ARG);
+        }
+        const int sum = __reduce_add_sync(0xffffffffu, n), mx = __reduce_max_sync(0xffffffffu, n);
+        if (lane == 0) {
+            s_scan[warp] = sum;
+            s_max[warp] = mx;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < DEC_WARPS; ++i) {
+            total += s_scan[i];
+            longest = max(longest, s_max[i]);
+        }
+        __syncthreads();
+    }
+    total *= p.H_kv;
+    // CTAs in use: no more than there are chunks, nor than leave a pair in DEC_MAX_SPLITS pieces
+    const int64_t active = min(min(static_cast<int64_t>(gridDim.x), total), max(static_cast<int64_t>(1), DEC_MAX_SPLITS * total / longest));
+    if (blockIdx.x >= active) return;
+    int64_t at = blockIdx.x * total / active;
+    const int64_t end = (blockIdx.x + 1) * total / active;
+    auto cta_of = [&](int64_t chunk) { return static_cast<int>(((chunk + 1) * active - 1) / total); };
+
+    // the entry that chunk `at` belongs to, and the first chunk of that entry
+    int e = 0;
+    int64_t e_first = 0;
+    {
+        int64_t base = 0;
+        for (int e0 = 0; e0 < p.E; e0 += DEC_THREADS) {
+            const int i = e0 + threadIdx.x;
+            int n = i < p.E ? chunks_of(context(i)) : 0, incl = n;
+#pragma unroll
+            for (int k = 1; k < 32; k <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, k);
+                if (lane >= k) incl += v;
+            }
+            if (lane == 31) s_scan[warp] = incl;
+            if (threadIdx.x == 0) s_at[0] = -1;
+            __syncthreads();
+            int before = incl - n, all = 0;
+#pragma unroll
+            for (int k = 0; k < DEC_WARPS; ++k) {
+                if (k < warp) before += s_scan[k];
+                all += s_scan[k];
+            }
+            const int64_t first = (base + before) * p.H_kv, last = first + static_cast<int64_t>(n) * p.H_kv;
+            if (n > 0 && at >= first && at < last) {
+                s_at[0] = i;
+                s_at[1] = static_cast<int>(at - first);
+            }
+            __syncthreads();
+            const bool found = s_at[0] >= 0;
+            if (found) {
+                e = s_at[0];
+                e_first = at - s_at[1];
+                break;
+            }
+            base += all;
+        }
+        __syncthreads();
+    }
+
+    while (at < end) {
+        const int ctx = context(e);
+        const int n = chunks_of(ctx);
+        const int kvh = static_cast<int>((at - e_first) / n);
+        const int64_t pair_first = e_first + static_cast<int64_t>(kvh) * n, pair_end = pair_first + n;
+        const int64_t stop = min(end, pair_end);
+        // this CTA's positions [pos0, pos1) of the pair
+        const int pos0 = static_cast<int>(at - pair_first) * CHUNK;
+        const int pos1 = min(ctx, static_cast<int>(stop - pair_first) * CHUNK);
+
+        // ---- q: the column operand (heads as columns), k-step j of chunk q4 + 4c: dims 16 (q4 + 4c) + 4 (j % 4) ..
+        uint32_t qb[4 * KC][2];
+        float back = 1.f;  // what q's scaling took off
+        {
+            const T *qp = static_cast<const T *>(p.q) + e * p.q_st + static_cast<int64_t>(kvh * G + r0) * p.q_sh;
+            uint32_t raw[8 * KC];
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r0 < G) v = *reinterpret_cast<const uint4 *>(qp + 16 * (q4 + 4 * c) + 8 * i);
+                    raw[8 * c + 4 * i] = v.x;
+                    raw[8 * c + 4 * i + 1] = v.y;
+                    raw[8 * c + 4 * i + 2] = v.z;
+                    raw[8 * c + 4 * i + 3] = v.w;
+                }
+            if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+                for (int i = 0; i < 8 * KC; ++i) qb[i / 2][i % 2] = raw[i];
+            } else {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8 * KC; ++i) {
+                    const float2 f = bf16x2_to_f32x2(raw[i]);
+                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^-k and 2^k with top / 2^k in [1, 2); 1 for zero and what is not finite
+                int k = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+                k = top > 0.f && k < 128 ? max(-120, min(k, 120)) : 0;
+                const float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+                back = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+#pragma unroll
+                for (int i = 0; i < 8 * KC; ++i) {
+                    const float2 f = bf16x2_to_f32x2(raw[i]);
+                    qb[i / 2][i % 2] = half2_of(f.x * down, f.y * down);
+                }
+            }
+        }
+        // this thread's columns of S^T: heads 2 q4 and 2 q4 + 1
+        const float c0 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * q4);
+        const float c1 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * q4 + 4);
+
+        float m0 = M_NONE, m1 = M_NONE, l0 = 0.f, l1 = 0.f;
+        float acc[MT][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+
+        // ---- pages: lane 2 U i + g holds those of group g (8 positions) of this warp's tile 16/U window + i
+        constexpr int WIN = 16 / U;  // tiles of a window
+        const int *table = p.block_table + e * p.bt_stride;
+        const int tiles = pos1 > pos0 ? (pos1 - pos0 + TILE - 1) / TILE : 0;
+        const int mine = tiles > warp ? (tiles - warp + DEC_WARPS - 1) / DEC_WARPS : 0;  // tiles warp, warp + 4, ...
+        auto tile_pos = [&](int i) { return pos0 + (warp + i * DEC_WARPS) * TILE; };
+        auto page_of = [&](int pos) {  // block id, -1 where there is nothing to read
+            int b = -1;
+            if (pos < pos1) {
+                b = __ldcg(table + pos / p.block_size);
+                if (b < 0 || b >= p.num_blocks) {
+                    report_status(LSE_ERR_INVALID_ARG);
+                    b = -1;
+                }
+            }
+            return b;
+        };
+        int win_blk = -1, nxt_blk = -1;  // block id
+        int win_row = -1;                // first row of the group in the pool / 8, -1: nothing to read
+        float win_k = 0.f, win_v = 0.f;
+        auto group_pos = [&](int window) { return tile_pos(window * WIN + lane / (2 * U)) + 8 * (lane % (2 * U)); };
+        auto lookup = [&](int window) {
+            return window * WIN + lane / (2 * U) < mine ? page_of(group_pos(window)) : -1;
+        };
+        auto scales = [&](int blk, float &k, float &v) {
+            const int64_t cell = static_cast<int64_t>(max(blk, 0)) * p.H_kv + kvh;
+            k = blk >= 0 ? __ldcg(p.k_scale + cell) : 0.f;
+            v = blk >= 0 ? __ldcg(p.v_scale + cell) : 0.f;
+        };
+        auto enter = [&](int window) {  // win_blk's other fields
+            scales(win_blk, win_k, win_v);
+            const int per = p.block_size >> 3;
+            win_row = win_blk < 0 ? -1 : (win_blk * p.H_kv + kvh) * per + (group_pos(window) >> 3) % per;
+        };
+
+        uint4 kr[U][2][KC];       // K rows r0, r0 + 8 of each 16 positions
+        uint32_t vr[U][4][VW];    // V rows 2 q4, 2 q4 + 1, + 8, + 9
+        float sk[U][2], sv[U][2];  // scales of positions r0 and r0 + 8
+        unsigned dead = 0;        // bit 2 u + i: positions that are not to be read
+        auto load_k = [&](uint4 (&dst)[KC], const int8_t *row) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) dst[c] = ld_stream16(row + 16 * (q4 + 4 * c));
+        };
+        auto load_v = [&](uint32_t (&dst)[VW], const int8_t *row) {
+            if constexpr (VW == 4) {
+                const uint4 v = ld_stream16(row + 16 * r0);
+                dst[0] = v.x; dst[1] = v.y; dst[2] = v.z; dst[3] = v.w;
+            } else {
+                const uint2 v = ld_stream8(row + 8 * r0);
+                dst[0] = v.x; dst[1] = v.y;
+            }
+        };
+        // Loads of tile i.  `k_out` etc. are the buffers of the next tile.
+        int64_t v_base[U][2];
+        int v_rows[U][4];
+        auto fetch_k = [&](int i, uint4 (&k)[U][2][KC], float (&a)[U][2], float (&b)[U][2], unsigned &gone) {
+            gone = 0;
+            if constexpr (PAGED8) {
+                if (i % WIN == 0 && i > 0) {
+                    win_blk = nxt_blk;
+                    nxt_blk = lookup(i / WIN + 1);
+                    enter(i / WIN);
+                }
+#pragma unroll
+                for (int g = 0; g < 2 * U; ++g) {
+                    const int src = (i % WIN) * 2 * U + g;
+                    const int row8 = __shfl_sync(0xffffffffu, win_row, src);
+                    a[g / 2][g % 2] = __shfl_sync(0xffffffffu, win_k, src);
+                    b[g / 2][g % 2] = __shfl_sync(0xffffffffu, win_v, src);
+                    if (row8 < 0) gone |= 1u << g;
+                    const int64_t base = static_cast<int64_t>(max(row8, 0)) * (8 * D);
+                    v_base[g / 2][g % 2] = base;
+                    load_k(k[g / 2][g % 2], p.k_pool + base + r0 * D);
+                }
+            } else {
+                // lane j: position pos + j
+                const int pos = tile_pos(i);
+                const int blk = lane < TILE ? page_of(pos + lane) : -1;
+                float ks, vs;
+                scales(blk, ks, vs);
+                const unsigned ok = __ballot_sync(0xffffffffu, blk >= 0);
+                const int row = max(blk, 0);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int j = 16 * u + 8 * h + r0;
+                        a[u][h] = __shfl_sync(0xffffffffu, ks, j);
+                        b[u][h] = __shfl_sync(0xffffffffu, vs, j);
+                        if (!((ok >> j) & 1u)) gone |= 1u << (2 * u + h);
+                        const int64_t cell = static_cast<int64_t>(__shfl_sync(0xffffffffu, row, j)) * p.H_kv + kvh;
+                        load_k(k[u][h], p.k_pool + (cell * p.block_size + (pos + j) % p.block_size) * D);
+                    }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) v_rows[u][h] = __shfl_sync(0xffffffffu, row, 16 * u + 8 * (h >> 1) + 2 * q4 + (h & 1));
+            }
+        };
+        auto fetch_v = [&](int i, uint32_t (&v)[U][4][VW]) {
+            [[maybe_unused]] const int pos = tile_pos(i);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    if constexpr (PAGED8) {
+                        load_v(v[u][h], p.v_pool + v_base[u][h >> 1] + (2 * q4 + (h & 1)) * D);
+                    } else {
+                        const int j = 16 * u + 8 * (h >> 1) + 2 * q4 + (h & 1);
+                        const int64_t cell = static_cast<int64_t>(v_rows[u][h]) * p.H_kv + kvh;
+                        load_v(v[u][h], p.v_pool + (cell * p.block_size + (pos + j) % p.block_size) * D);
+                    }
+                }
+        };
+
+        if (mine > 0) {
+            if constexpr (PAGED8) {
+                win_blk = lookup(0);
+                nxt_blk = lookup(1);
+                enter(0);
+            }
+            fetch_k(0, kr, sk, sv, dead);
+            fetch_v(0, vr);
+        }
+        for (int i = 0; i < mine; ++i) {
+            uint4 kn[U][2][KC];
+            float skn[U][2], svn[U][2];
+            unsigned deadn = 0;
+            if (i + 1 < mine) fetch_k(i + 1, kn, skn, svn, deadn);
+            // ---- S^T = K Q^T -------------------------------------------------------------
+            float s[U][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float odd[4] = {0.f, 0.f, 0.f, 0.f};
+                s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const uint32_t a[4] = {kr[u][0][c].x, kr[u][0][c].y, kr[u][0][c].z, kr[u][0][c].w};
+                    const uint32_t b[4] = {kr[u][1][c].x, kr[u][1][c].y, kr[u][1][c].z, kr[u][1][c].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t x = a[j] ^ 0x80808080u, y = b[j] ^ 0x80808080u;
+                        mma_f16((j & 1) ? odd : s[u], codes_lo(x), codes_lo(y), codes_hi(x), codes_hi(y), qb[4 * c + j][0],
+                                qb[4 * c + j][1]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[u][j] += odd[j];
+            }
+            // ---- scores in base 2, masks --------------------------------------------------
+            const int pos = tile_pos(i);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    s[u][2 * h] *= c0 * sk[u][h];
+                    s[u][2 * h + 1] *= c1 * sk[u][h];
+                }
+            const bool masks = pos + TILE > pos1 || __any_sync(0xffffffffu, dead != 0);
+            if (masks) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (((dead >> (2 * u + h)) & 1u) || pos + 16 * u + 8 * h + r0 >= pos1)
+                            s[u][2 * h] = s[u][2 * h + 1] = -INFINITY;
+            }
+            // ---- does anything exceed M by 2^6? -------------------------------------------
+            float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float lv = __log2f(fmaxf(fabsf(sv[u][h]), 7.8886e-31f));  // 2^-100: p stays below 2^106
+                    x0 = fmaxf(x0, s[u][2 * h] + lv);
+                    x1 = fmaxf(x1, s[u][2 * h + 1] + lv);
+                }
+            if (__any_sync(0xffffffffu, x0 > m0 + 6.f || x1 > m1 + 6.f)) {
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, k));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, k));
+                }
+                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                const float f0 = ex2_approx(m0 - n0), f1 = ex2_approx(m1 - n1);
+                m0 = n0;
+                m1 = n1;
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    acc[t][0] *= f0;
+                    acc[t][1] *= f1;
+                    acc[t][2] *= f0;
+                    acc[t][3] *= f1;
+                }
+            }
+            // ---- weights, and P^T as the column operand ------------------------------------
+            uint32_t pb[U][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float w0 = ex2_approx(s[u][2 * h] - m0), w1 = ex2_approx(s[u][2 * h + 1] - m1);
+                    l0 += w0;
+                    l1 += w1;
+                    // a masked position has weight 0, whatever its page's scale
+                    float y0 = w0 * sv[u][h], y1 = w1 * sv[u][h];
+                    if (masks && s[u][2 * h] == -INFINITY) y0 = y1 = 0.f;
+                    pb[u][h] = movm_trans(half2_of(y0, y1));
+                }
+            // ---- O^T += V^T P^T -------------------------------------------------------------
+            uint32_t vn[U][4][VW];
+            if (i + 1 < mine) fetch_v(i + 1, vn);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int x = 0; x < VW; ++x) {
+                    const uint32_t a = vr[u][0][x] ^ 0x80808080u, b = vr[u][1][x] ^ 0x80808080u;
+                    const uint32_t c = vr[u][2][x] ^ 0x80808080u, d = vr[u][3][x] ^ 0x80808080u;
+                    const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+                    const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+                    mma_f16(acc[2 * x], codes_lo(ab0), codes_hi(ab0), codes_lo(cd0), codes_hi(cd0), pb[u][0], pb[u][1]);
+                    mma_f16(acc[2 * x + 1], codes_lo(ab1), codes_hi(ab1), codes_lo(cd1), codes_hi(cd1), pb[u][0], pb[u][1]);
+                }
+            if (i + 1 < mine) {
+                dead = deadn;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        sk[u][h] = skn[u][h];
+                        sv[u][h] = svn[u][h];
+#pragma unroll
+                        for (int c = 0; c < KC; ++c) kr[u][h][c] = kn[u][h][c];
+                    }
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+#pragma unroll
+                        for (int x = 0; x < VW; ++x) vr[u][h][x] = vn[u][h][x];
+                }
+            }
+        }
+
+        // ---- the four warps' sums -------------------------------------------------------------
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, k);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, k);
+        }
+        __syncthreads();  // the previous pair's readers are done with the buffers
+        if (2 * q4 < G) {
+            const int h0 = 2 * q4;
+            if (r0 == 0) {
+                s_ml[warp][h0][0] = m0;
+                s_ml[warp][h0][1] = l0;
+                if (h0 + 1 < G) {
+                    s_ml[warp][h0 + 1][0] = m1;
+                    s_ml[warp][h0 + 1][1] = l1;
+                }
+            }
+            // dim (D / 8) r0 + k is kept at 8 k + r0: no bank conflicts here
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                s_acc[warp][h0][16 * t + r0] = acc[t][0];
+                s_acc[warp][h0][16 * t + 8 + r0] = acc[t][2];
+                if (h0 + 1 < G) {
+                    s_acc[warp][h0 + 1][16 * t + r0] = acc[t][1];
+                    s_acc[warp][h0 + 1][16 * t + 8 + r0] = acc[t][3];
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = at == pair_first && stop == pair_end;
+        const int slot = 2 * blockIdx.x + (at == pair_first ? 1 : 0);
+        T *o = static_cast<T *>(p.o) + e * p.o_st + static_cast<int64_t>(kvh) * G * p.o_sh;
+        for (int i = threadIdx.x; i < G * D; i += DEC_THREADS) {
+            const int h = i / D, d = i % D, k = (d % (D / 8)) * 8 + d / (D / 8);
+            float M = s_ml[0][h][0], L = 0.f, A = 0.f;
+#pragma unroll
+            for (int x = 1; x < DEC_WARPS; ++x) M = fmaxf(M, s_ml[x][h][0]);
+#pragma unroll
+            for (int x = 0; x < DEC_WARPS; ++x) {
+                const float f = ex2_approx(s_ml[x][h][0] - M);
+                L += s_ml[x][h][1] * f;
+                A += s_acc[x][h][k] * f;
+            }
+            if (whole) {
+                o[h * p.o_sh + d] = from_float<T>(L != 0.f ? A / L : 0.f);
+            } else {
+                w.acc[static_cast<int64_t>(slot) * (G * D) + i] = A;
+                if (d == 0) {
+                    w.ml[(static_cast<int64_t>(slot) * G + h) * 2] = M;
+                    w.ml[(static_cast<int64_t>(slot) * G + h) * 2 + 1] = L;
+                }
+            }
+        }
+        if (!whole) {
+            // ---- publish; the last of the pair's CTAs joins their sums in the order of the positions
+            const int first = cta_of(pair_first), pieces = cta_of(pair_end - 1) - first + 1;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const int old = atomicAdd(w.counters + first, 1);
+                s_at[2] = old == pieces - 1;
+                if (old == pieces - 1) w.counters[first] = 0;  // ready for the next launch
+            }
+            __syncthreads();
+            if (s_at[2]) {
+                __threadfence();
+                auto slot_of = [&](int i) { return static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)); };
+                for (int h = warp; h < G; h += DEC_WARPS) {
+                    float M = M_NONE;
+                    for (int i = lane; i < pieces; i += 32) M = fmaxf(M, __ldcg(w.ml + (slot_of(i) * G + h) * 2));
+#pragma unroll
+                    for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+                    float L = 0.f;
+                    for (int i = lane; i < pieces; i += 32) {
+                        const float f = ex2_approx(__ldcg(w.ml + (slot_of(i) * G + h) * 2) - M);
+                        s_w[i][h] = f;
+                        L += f * __ldcg(w.ml + (slot_of(i) * G + h) * 2 + 1);
+                    }
+#pragma unroll
+                    for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+                    if (lane == 0) s_l[h] = L;
+                }
+                __syncthreads();
+                for (int i = 4 * threadIdx.x; i < G * D; i += 4 * DEC_THREADS) {
+                    const int h = i / D;
+                    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                    for (int k = 0; k < pieces; ++k) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(w.acc + slot_of(k) * (G * D) + i));
+                        const float f = s_w[k][h];
+                        A.x = fmaf(v.x, f, A.x);
+                        A.y = fmaf(v.y, f, A.y);
+                        A.z = fmaf(v.z, f, A.z);
+                        A.w = fmaf(v.w, f, A.w);
+                    }
+                    const float L = s_l[h], inv = L != 0.f ? 1.f / L : 0.f;
+                    T *dst = o + h * p.o_sh + i % D;
+                    dst[0] = from_float<T>(A.x * inv);
+                    dst[1] = from_float<T>(A.y * inv);
+                    dst[2] = from_float<T>(A.z * inv);
+                    dst[3] = from_float<T>(A.w * inv);
+                }
+                __syncthreads();
+            }
+        }
+        at = stop;
+        if (at == e_first + static_cast<int64_t>(n) * p.H_kv) {
+            e_first = at;
+            ++e;
+        }
+    }
+}
+
+}  // namespace kv8
+}  // namespace lse

@@ -23,6 +23,7 @@
 
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <utility>
 
 #include "../../include/lse_int8.h"
@@ -183,6 +184,30 @@ at::Tensor rows16(const at::Tensor &x) {
     return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
+// Scratch whose counters every call leaves at zero: one zeroed buffer per device, stream and
+// kernel, kept between calls and grown (never inside a capture) when a call needs more.  A
+// stream capture has a buffer of its own, allocated and zeroed by the captured work, so that a
+// replay shares nothing with eager calls on any stream.
+at::Tensor counters_workspace(int which, size_t bytes, const at::Tensor &like, cudaStream_t stream) {
+    static std::mutex lock;
+    static auto &kept = *new std::map<std::tuple<int, int, cudaStream_t>, at::Tensor>();  // alive to the process's end
+    static auto &captured = *new std::map<std::tuple<int, int, cudaStream_t>, std::pair<unsigned long long, at::Tensor>>();
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
+    const auto key = std::make_tuple(which, static_cast<int>(like.get_device()), stream);
+    const auto fresh = [&] { return at::zeros({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)); };
+    const std::lock_guard<std::mutex> guard(lock);
+    if (status == cudaStreamCaptureStatusActive) {
+        auto &c = captured[key];
+        if (!c.second.defined() || c.first != id || static_cast<size_t>(c.second.numel()) < bytes) c = {id, fresh()};
+        return c.second;
+    }
+    at::Tensor &t = kept[key];
+    if (!t.defined() || static_cast<size_t>(t.numel()) < bytes) t = fresh();
+    return t;
+}
+
 at::Tensor kv8_rope_append(const at::Tensor &qkv, int64_t n_heads, const at::Tensor &k, const at::Tensor &v,
                            const at::Tensor &k_scale, const at::Tensor &v_scale, const at::Tensor &block_table,
                            const at::Tensor &query_offset, const at::Tensor &q_start, const at::Tensor &q_len,
@@ -271,19 +296,22 @@ at::Tensor kv8_decode_attention(const at::Tensor &q, const at::Tensor &k, const 
     check_table(block_table, dev, what);
     const int dt = dtype_code(q);
     const int64_t E = block_table.size(0);
-    TORCH_CHECK(q.dim() == 3 && q.size(0) == E && q.size(2) == c.D(), what, ": q must be [E, H, D] with the cache's D");
+    TORCH_CHECK(q.dim() == 3 && q.size(0) == E && q.size(1) % c.H_kv() == 0 && q.size(2) == c.D(), what, ": q must be [E, H, D] with the cache's D");
     check_i32(context_len, E, dev, what, "context_len");
     c10::cuda::CUDAGuard guard(dev);
     init_device(dev.index());
     at::Tensor o = at::empty({E, q.size(1), c.D()}, q.options());
     if (E == 0 || q.size(1) == 0) return o;
     const at::Tensor x = rows16(q);
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const size_t ws_bytes = lse_kv8_decode_attention_workspace(q.size(1), c.H_kv(), c.D());
+    const at::Tensor ws = counters_workspace(0, ws_bytes, q, st);
     check_launch(lse_kv8_decode_attention(x.data_ptr(), dt, E, q.size(1), c.D(), x.stride(0), x.stride(1), k.data_ptr<int8_t>(),
                                           v.data_ptr<int8_t>(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
                                           c.num_blocks(), c.block_size(), c.H_kv(), block_table.data_ptr<int>(),
                                           block_table.stride(0), block_table.size(1), context_len.data_ptr<int>(),
-                                          static_cast<float>(scale), o.data_ptr(), o.stride(0), o.stride(1), nullptr, 0,
-                                          at::cuda::getCurrentCUDAStream(dev.index()).stream()),
+                                          static_cast<float>(scale), o.data_ptr(), o.stride(0), o.stride(1), ws.data_ptr(),
+                                          ws_bytes, st),
                  "lse_kv8_decode_attention");
     return o;
 }
