@@ -111,7 +111,7 @@ int launch_rows(const kv8::AttnParams &p, int sms, cudaStream_t st) {
 }
 
 // Resident CTAs per SM of the decode kernel (its launch bounds) and so the launch's grid.
-constexpr int kDecodePerSm = 3;
+constexpr int kDecodePerSm = 4;
 
 size_t decode_counter_bytes(int sms) { return (static_cast<size_t>(kDecodePerSm) * sms * sizeof(int) + 255) / 256 * 256; }
 
@@ -119,12 +119,12 @@ template <int D, int G, typename T>
 int launch_decode(const kv8::AttnParams &p, const kv8::DecodeWork &w, int sms, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    const bool paged8 = p.block_size % 8 == 0;
-    const int grid = kDecodePerSm * sms;
-    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(grid)), dim3(kv8::DEC_THREADS), 0, st);
-    return finish(paged8 ? cudaLaunchKernelEx(&cfg, kv8::decode_kernel<D, G, T, true>, p, w)
-                         : cudaLaunchKernelEx(&cfg, kv8::decode_kernel<D, G, T, false>, p, w),
-                  "kv8_decode_attention launch");
+    const auto kernel = p.block_size % 8 == 0 ? kv8::decode_kernel<D, G, T, true> : kv8::decode_kernel<D, G, T, false>;
+    constexpr int smem = kv8::DEC_SMEM<D>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return finish(e, "kv8_decode_attention attributes");
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(kDecodePerSm * sms)), dim3(kv8::DEC_THREADS), smem, st);
+    return finish(cudaLaunchKernelEx(&cfg, kernel, p, w), "kv8_decode_attention launch");
 }
 
 template <int D, typename T>

@@ -33,6 +33,7 @@ namespace kv8 {
 
 constexpr int DEC_WARPS = 4;
 constexpr int DEC_THREADS = DEC_WARPS * 32;
+constexpr int DEC_STAGES = 3;       // tiles in flight per warp
 constexpr int DEC_MAX_SPLITS = 64;  // CTAs that share a pair, at most (+ 1 by rounding)
 
 // A tile is what one warp takes at a time; a chunk one tile for each warp.
@@ -40,6 +41,8 @@ template <int D>
 constexpr int DEC_TILE = 16 * (128 / D);
 template <int D>
 constexpr int DEC_CHUNK = DEC_WARPS * DEC_TILE<D>;
+template <int D>
+constexpr int DEC_SMEM = DEC_WARPS * DEC_STAGES * 2 * DEC_TILE<D> * D;
 
 struct DecodeWork {
     int *counters;  // [grid] arrivals at the pair that starts last in a CTA, zero between launches
@@ -52,14 +55,12 @@ __device__ __forceinline__ float ex2_approx(float x) {  // 2^x, relative error 2
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint4 ld_stream16(const int8_t *p) {
-    uint4 r;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-    return r;
+__device__ __forceinline__ void copy16(uint32_t dst, const int8_t *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 ld_stream8(const int8_t *p) {
-    uint2 r;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(p) : "memory");
     return r;
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -93,18 +94,24 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t u) {
 // PAGED8: block_size is a multiple of 8, so that 8 consecutive positions share a page and its scales;
 // otherwise every position looks its page up for itself.
 template <int D, int G, typename T, bool PAGED8>
-__global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams p, const DecodeWork w) {
+__global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams p, const DecodeWork w) {
     constexpr int U = 128 / D;          // 16-position MMA rows of a tile
     constexpr int TILE = DEC_TILE<D>, CHUNK = DEC_CHUNK<D>;
     constexpr int KC = D / 64;          // 16-byte chunks of a K row per thread
     constexpr int VW = D / 32;          // words of a V row per thread
+    constexpr int VB = 4 * VW;          // ... bytes
     constexpr int MT = D / 16;          // 16-dim row tiles of O^T
+    constexpr int WIN = 16 / U;         // tiles of a window of page look-ups
+    constexpr int STAGES = DEC_STAGES, K_BYTES = TILE * D, STAGE = 2 * K_BYTES;
     constexpr float M_NONE = -1e30f;    // below every score; finite, so that 2^(-inf - M) is 0
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r0 = lane >> 2, q4 = lane & 3;
     const int64_t table_positions = static_cast<int64_t>(p.bt_cols) * p.block_size;
 
-    __shared__ float s_acc[DEC_WARPS][G][D + 4];
+    extern __shared__ __align__(16) uint8_t s_ring[];  // [DEC_WARPS][STAGES][K, V]; between pairs the warps' sums
+    auto s_acc = reinterpret_cast<float (*)[G][D + 4]>(s_ring);
+    static_assert(G * (D + 4) * 4 <= STAGES * STAGE, "the sums fit the ring");
+    __shared__ float s_scale[PAGED8 ? 1 : DEC_WARPS][PAGED8 ? 1 : STAGES][PAGED8 ? 1 : TILE][2];
     __shared__ float s_ml[DEC_WARPS][G][2];
     __shared__ float s_w[DEC_MAX_SPLITS + 2][G], s_l[G];
     __shared__ int s_scan[DEC_WARPS], s_max[DEC_WARPS];
@@ -116,6 +123,21 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
     auto context = [&](int e) {  // positions of entry e, cut to its table
         const int c = __ldcg(p.context_len + e);
         return static_cast<int>(min(static_cast<int64_t>(max(c, 0)), table_positions));
+    };
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) + warp * STAGES * STAGE;
+    int window = 0;  // of the tile being consumed
+    auto slot_window = [](int i) { return i / WIN; };
+    auto copy_v = [](uint32_t dst, const int8_t *src) {
+        if constexpr (VW == 4) copy16(dst, src);
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    };
+    auto lds_v = [](uint32_t (&v)[VW], uint32_t src) {
+        if constexpr (VW == 4) {
+            const uint4 x = lds16(src);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(src) : "memory");
+        }
     };
     auto chunks_of = [](int ctx) { return max(1, (ctx + CHUNK - 1) / CHUNK); };
 
@@ -250,8 +272,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 
-        // ---- pages: lane 2 U i + g holds those of group g (8 positions) of this warp's tile 16/U window + i
-        constexpr int WIN = 16 / U;  // tiles of a window
+        // ---- pages: lane 2 U i + g holds those of group g (8 positions) of tile i of a window of this warp's tiles
         const int *table = p.block_table + e * p.bt_stride;
         const int tiles = pos1 > pos0 ? (pos1 - pos0 + TILE - 1) / TILE : 0;
         const int mine = tiles > warp ? (tiles - warp + DEC_WARPS - 1) / DEC_WARPS : 0;  // tiles warp, warp + 4, ...
@@ -267,118 +288,95 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
             }
             return b;
         };
-        int win_blk = -1, nxt_blk = -1;  // block id
-        int win_row = -1;                // first row of the group in the pool / 8, -1: nothing to read
-        float win_k = 0.f, win_v = 0.f;
-        auto group_pos = [&](int window) { return tile_pos(window * WIN + lane / (2 * U)) + 8 * (lane % (2 * U)); };
-        auto lookup = [&](int window) {
-            return window * WIN + lane / (2 * U) < mine ? page_of(group_pos(window)) : -1;
-        };
         auto scales = [&](int blk, float &k, float &v) {
             const int64_t cell = static_cast<int64_t>(max(blk, 0)) * p.H_kv + kvh;
             k = blk >= 0 ? __ldcg(p.k_scale + cell) : 0.f;
             v = blk >= 0 ? __ldcg(p.v_scale + cell) : 0.f;
         };
-        auto enter = [&](int window) {  // win_blk's other fields
-            scales(win_blk, win_k, win_v);
+        auto group_pos = [&](int window) { return tile_pos(window * WIN + lane / (2 * U)) + 8 * (lane % (2 * U)); };
+        // The window being consumed, the next one (its loads in flight) and the block ids of the one after
+        int row_now = -1, row_next = -1, blk_after = -1;  // a group's first row in the pool / 8, -1: nothing to read
+        float k_now = 0.f, v_now = 0.f, k_next = 0.f, v_next = 0.f;
+        auto lookup = [&](int window) { return window * WIN + lane / (2 * U) < mine ? page_of(group_pos(window)) : -1; };
+        auto next_window = [&](int window) {  // fills *_next for `window` from blk_after
+            scales(blk_after, k_next, v_next);
             const int per = p.block_size >> 3;
-            win_row = win_blk < 0 ? -1 : (win_blk * p.H_kv + kvh) * per + (group_pos(window) >> 3) % per;
+            row_next = blk_after < 0 ? -1 : (blk_after * p.H_kv + kvh) * per + (group_pos(window) >> 3) % per;
+            blk_after = lookup(window + 1);
         };
 
-        uint4 kr[U][2][KC];       // K rows r0, r0 + 8 of each 16 positions
-        uint32_t vr[U][4][VW];    // V rows 2 q4, 2 q4 + 1, + 8, + 9
-        float sk[U][2], sv[U][2];  // scales of positions r0 and r0 + 8
-        unsigned dead = 0;        // bit 2 u + i: positions that are not to be read
-        auto load_k = [&](uint4 (&dst)[KC], const int8_t *row) {
-#pragma unroll
-            for (int c = 0; c < KC; ++c) dst[c] = ld_stream16(row + 16 * (q4 + 4 * c));
-        };
-        auto load_v = [&](uint32_t (&dst)[VW], const int8_t *row) {
-            if constexpr (VW == 4) {
-                const uint4 v = ld_stream16(row + 16 * r0);
-                dst[0] = v.x; dst[1] = v.y; dst[2] = v.z; dst[3] = v.w;
-            } else {
-                const uint2 v = ld_stream8(row + 8 * r0);
-                dst[0] = v.x; dst[1] = v.y;
-            }
-        };
-        // Loads of tile i.  `k_out` etc. are the buffers of the next tile.
-        int64_t v_base[U][2];
-        int v_rows[U][4];
-        auto fetch_k = [&](int i, uint4 (&k)[U][2][KC], float (&a)[U][2], float (&b)[U][2], unsigned &gone) {
-            gone = 0;
-            if constexpr (PAGED8) {
-                if (i % WIN == 0 && i > 0) {
-                    win_blk = nxt_blk;
-                    nxt_blk = lookup(i / WIN + 1);
-                    enter(i / WIN);
+        // Copies of tile i into its slot of the ring, thread-private: each thread copies what it will read.
+        auto issue = [&](int i, int slot) {
+            const uint32_t dst = ring + slot * STAGE;
+            if (i < mine) {
+                const int pos = tile_pos(i);
+                [[maybe_unused]] int row = 0;
+                if constexpr (!PAGED8) {  // lane j: position pos + j, its scales kept beside the ring
+                    const int blk = lane < TILE ? page_of(pos + lane) : -1;
+                    float ks, vs;
+                    scales(blk, ks, vs);
+                    if (lane < TILE) {
+                        s_scale[warp][slot][lane][0] = blk < 0 ? -INFINITY : ks;  // -inf: not to be read
+                        s_scale[warp][slot][lane][1] = vs;
+                    }
+                    row = max(blk, 0);
+                    __syncwarp();
                 }
 #pragma unroll
                 for (int g = 0; g < 2 * U; ++g) {
-                    const int src = (i % WIN) * 2 * U + g;
-                    const int row8 = __shfl_sync(0xffffffffu, win_row, src);
-                    a[g / 2][g % 2] = __shfl_sync(0xffffffffu, win_k, src);
-                    b[g / 2][g % 2] = __shfl_sync(0xffffffffu, win_v, src);
-                    if (row8 < 0) gone |= 1u << g;
-                    const int64_t base = static_cast<int64_t>(max(row8, 0)) * (8 * D);
-                    v_base[g / 2][g % 2] = base;
-                    load_k(k[g / 2][g % 2], p.k_pool + base + r0 * D);
-                }
-            } else {
-                // lane j: position pos + j
-                const int pos = tile_pos(i);
-                const int blk = lane < TILE ? page_of(pos + lane) : -1;
-                float ks, vs;
-                scales(blk, ks, vs);
-                const unsigned ok = __ballot_sync(0xffffffffu, blk >= 0);
-                const int row = max(blk, 0);
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int j = 16 * u + 8 * h + r0;
-                        a[u][h] = __shfl_sync(0xffffffffu, ks, j);
-                        b[u][h] = __shfl_sync(0xffffffffu, vs, j);
-                        if (!((ok >> j) & 1u)) gone |= 1u << (2 * u + h);
-                        const int64_t cell = static_cast<int64_t>(__shfl_sync(0xffffffffu, row, j)) * p.H_kv + kvh;
-                        load_k(k[u][h], p.k_pool + (cell * p.block_size + (pos + j) % p.block_size) * D);
-                    }
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) v_rows[u][h] = __shfl_sync(0xffffffffu, row, 16 * u + 8 * (h >> 1) + 2 * q4 + (h & 1));
-            }
-        };
-        auto fetch_v = [&](int i, uint32_t (&v)[U][4][VW]) {
-            [[maybe_unused]] const int pos = tile_pos(i);
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
                     if constexpr (PAGED8) {
-                        load_v(v[u][h], p.v_pool + v_base[u][h >> 1] + (2 * q4 + (h & 1)) * D);
+                        const bool ahead = slot_window(i) != window;
+                        const int src = (i % WIN) * 2 * U + g;
+                        const int row8 = max(__shfl_sync(0xffffffffu, ahead ? row_next : row_now, src), 0);
+                        const int64_t base = static_cast<int64_t>(row8) * (8 * D);
+#pragma unroll
+                        for (int c = 0; c < KC; ++c)
+                            copy16(dst + (g * KC + c) * 512 + lane * 16, p.k_pool + base + r0 * D + 16 * (q4 + 4 * c));
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+                            copy_v(dst + K_BYTES + (2 * g + y) * (32 * VB) + lane * VB, p.v_pool + base + (2 * q4 + y) * D + VB * r0);
                     } else {
-                        const int j = 16 * u + 8 * (h >> 1) + 2 * q4 + (h & 1);
-                        const int64_t cell = static_cast<int64_t>(v_rows[u][h]) * p.H_kv + kvh;
-                        load_v(v[u][h], p.v_pool + (cell * p.block_size + (pos + j) % p.block_size) * D);
+                        auto at_row = [&](int j) {
+                            const int64_t cell = static_cast<int64_t>(__shfl_sync(0xffffffffu, row, j)) * p.H_kv + kvh;
+                            return (cell * p.block_size + (pos + j) % p.block_size) * D;
+                        };
+                        const int64_t kb = at_row(8 * g + r0);
+#pragma unroll
+                        for (int c = 0; c < KC; ++c)
+                            copy16(dst + (g * KC + c) * 512 + lane * 16, p.k_pool + kb + 16 * (q4 + 4 * c));
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+                            copy_v(dst + K_BYTES + (2 * g + y) * (32 * VB) + lane * VB, p.v_pool + at_row(8 * g + 2 * q4 + y) + VB * r0);
                     }
                 }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
 
-        if (mine > 0) {
-            if constexpr (PAGED8) {
-                win_blk = lookup(0);
-                nxt_blk = lookup(1);
-                enter(0);
-            }
-            fetch_k(0, kr, sk, sv, dead);
-            fetch_v(0, vr);
+        window = 0;
+        if constexpr (PAGED8) {
+            blk_after = lookup(0);
+            next_window(0);
+            row_now = row_next;
+            k_now = k_next;
+            v_now = v_next;
+            next_window(1);
         }
+        for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
+        int slot = 0;
         for (int i = 0; i < mine; ++i) {
-            uint4 kn[U][2][KC];
-            float skn[U][2], svn[U][2];
-            unsigned deadn = 0;
-            if (i + 1 < mine) fetch_k(i + 1, kn, skn, svn, deadn);
+            if constexpr (PAGED8) {
+                if (i % WIN == 0 && i > 0) {
+                    ++window;
+                    row_now = row_next;
+                    k_now = k_next;
+                    v_now = v_next;
+                    next_window(window + 1);
+                }
+            }
+            issue(i + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            const uint32_t src = ring + slot * STAGE;
             // ---- S^T = K Q^T -------------------------------------------------------------
             float s[U][4];
 #pragma unroll
@@ -387,8 +385,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
                 s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
-                    const uint32_t a[4] = {kr[u][0][c].x, kr[u][0][c].y, kr[u][0][c].z, kr[u][0][c].w};
-                    const uint32_t b[4] = {kr[u][1][c].x, kr[u][1][c].y, kr[u][1][c].z, kr[u][1][c].w};
+                    const uint4 ka = lds16(src + (2 * u * KC + c) * 512 + lane * 16);
+                    const uint4 kb = lds16(src + ((2 * u + 1) * KC + c) * 512 + lane * 16);
+                    const uint32_t a[4] = {ka.x, ka.y, ka.z, ka.w}, b[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint32_t x = a[j] ^ 0x80808080u, y = b[j] ^ 0x80808080u;
@@ -401,21 +400,36 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
             }
             // ---- scores in base 2, masks --------------------------------------------------
             const int pos = tile_pos(i);
+            float sv[U][2];
+            bool dead = false;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    s[u][2 * h] *= c0 * sk[u][h];
-                    s[u][2 * h + 1] *= c1 * sk[u][h];
+                    float sk;
+                    bool gone;
+                    if constexpr (PAGED8) {
+                        const int lane_of = (i % WIN) * 2 * U + 2 * u + h;
+                        sk = __shfl_sync(0xffffffffu, k_now, lane_of);
+                        sv[u][h] = __shfl_sync(0xffffffffu, v_now, lane_of);
+                        gone = __shfl_sync(0xffffffffu, row_now, lane_of) < 0;
+                    } else {
+                        sk = s_scale[warp][slot][16 * u + 8 * h + r0][0];
+                        sv[u][h] = s_scale[warp][slot][16 * u + 8 * h + r0][1];
+                        gone = sk == -INFINITY;
+                    }
+                    s[u][2 * h] *= c0 * sk;
+                    s[u][2 * h + 1] *= c1 * sk;
+                    if (gone) s[u][2 * h] = s[u][2 * h + 1] = -INFINITY;
+                    dead |= gone;
                 }
-            const bool masks = pos + TILE > pos1 || __any_sync(0xffffffffu, dead != 0);
+            const bool masks = pos + TILE > pos1 || __any_sync(0xffffffffu, dead);
             if (masks) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        if (((dead >> (2 * u + h)) & 1u) || pos + 16 * u + 8 * h + r0 >= pos1)
-                            s[u][2 * h] = s[u][2 * h + 1] = -INFINITY;
+                        if (pos + 16 * u + 8 * h + r0 >= pos1) s[u][2 * h] = s[u][2 * h + 1] = -INFINITY;
             }
             // ---- does anything exceed M by 2^6? -------------------------------------------
             float x0 = -INFINITY, x1 = -INFINITY;
@@ -462,37 +476,25 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
                     pb[u][h] = movm_trans(half2_of(y0, y1));
                 }
             // ---- O^T += V^T P^T -------------------------------------------------------------
-            uint32_t vn[U][4][VW];
-            if (i + 1 < mine) fetch_v(i + 1, vn);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                uint32_t v[4][VW];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) lds_v(v[y], src + K_BYTES + (4 * u + y) * (32 * VB) + lane * VB);
 #pragma unroll
                 for (int x = 0; x < VW; ++x) {
-                    const uint32_t a = vr[u][0][x] ^ 0x80808080u, b = vr[u][1][x] ^ 0x80808080u;
-                    const uint32_t c = vr[u][2][x] ^ 0x80808080u, d = vr[u][3][x] ^ 0x80808080u;
+                    const uint32_t a = v[0][x] ^ 0x80808080u, b = v[1][x] ^ 0x80808080u;
+                    const uint32_t c = v[2][x] ^ 0x80808080u, d = v[3][x] ^ 0x80808080u;
                     const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
                     const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
                     mma_f16(acc[2 * x], codes_lo(ab0), codes_hi(ab0), codes_lo(cd0), codes_hi(cd0), pb[u][0], pb[u][1]);
                     mma_f16(acc[2 * x + 1], codes_lo(ab1), codes_hi(ab1), codes_lo(cd1), codes_hi(cd1), pb[u][0], pb[u][1]);
                 }
-            if (i + 1 < mine) {
-                dead = deadn;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        sk[u][h] = skn[u][h];
-                        sv[u][h] = svn[u][h];
-#pragma unroll
-                        for (int c = 0; c < KC; ++c) kr[u][h][c] = kn[u][h][c];
-                    }
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
-#pragma unroll
-                        for (int x = 0; x < VW; ++x) vr[u][h][x] = vn[u][h][x];
-                }
             }
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
+            if constexpr (!PAGED8) __syncwarp();  // the slot's scales are free for the next tile's
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
 
         // ---- the four warps' sums -------------------------------------------------------------
 #pragma unroll
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
             l0 += __shfl_xor_sync(0xffffffffu, l0, k);
             l1 += __shfl_xor_sync(0xffffffffu, l1, k);
         }
-        __syncthreads();  // the previous pair's readers are done with the buffers
+        __syncthreads();  // every warp is done with its part of the ring
         if (2 * q4 < G) {
             const int h0 = 2 * q4;
             if (r0 == 0) {
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
         }
         __syncthreads();
         const bool whole = at == pair_first && stop == pair_end;
-        const int slot = 2 * blockIdx.x + (at == pair_first ? 1 : 0);
+        const int piece = 2 * blockIdx.x + (at == pair_first ? 1 : 0);
         T *o = static_cast<T *>(p.o) + e * p.o_st + static_cast<int64_t>(kvh) * G * p.o_sh;
         for (int i = threadIdx.x; i < G * D; i += DEC_THREADS) {
             const int h = i / D, d = i % D, k = (d % (D / 8)) * 8 + d / (D / 8);
@@ -540,10 +542,10 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
             if (whole) {
                 o[h * p.o_sh + d] = from_float<T>(L != 0.f ? A / L : 0.f);
             } else {
-                w.acc[static_cast<int64_t>(slot) * (G * D) + i] = A;
+                w.acc[static_cast<int64_t>(piece) * (G * D) + i] = A;
                 if (d == 0) {
-                    w.ml[(static_cast<int64_t>(slot) * G + h) * 2] = M;
-                    w.ml[(static_cast<int64_t>(slot) * G + h) * 2 + 1] = L;
+                    w.ml[(static_cast<int64_t>(piece) * G + h) * 2] = M;
+                    w.ml[(static_cast<int64_t>(piece) * G + h) * 2 + 1] = L;
                 }
             }
         }
@@ -599,6 +601,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
                 __syncthreads();
             }
         }
+        __syncthreads();  // the ring is free for the next pair's copies
         at = stop;
         if (at == e_first + static_cast<int64_t>(n) * p.H_kv) {
             e_first = at;
