@@ -111,7 +111,7 @@ int launch_rows(const kv8::AttnParams &p, int sms, cudaStream_t st) {
 }
 
 // Resident CTAs per SM of the decode kernel (its launch bounds) and so the launch's grid.
-constexpr int kDecodePerSm = 4;
+constexpr int kDecodePerSm = 3;
 
 size_t decode_counter_bytes(int sms) { return (static_cast<size_t>(kDecodePerSm) * sms * sizeof(int) + 255) / 256 * 256; }
 

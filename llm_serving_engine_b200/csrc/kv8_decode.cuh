@@ -33,16 +33,17 @@ namespace kv8 {
 
 constexpr int DEC_WARPS = 4;
 constexpr int DEC_THREADS = DEC_WARPS * 32;
-constexpr int DEC_STAGES = 3;       // tiles in flight per warp
 constexpr int DEC_MAX_SPLITS = 64;  // CTAs that share a pair, at most (+ 1 by rounding)
 
 // A tile is what one warp takes at a time; a chunk one tile for each warp.
 template <int D>
-constexpr int DEC_TILE = 16 * (128 / D);
+constexpr int DEC_TILE = 32;
 template <int D>
 constexpr int DEC_CHUNK = DEC_WARPS * DEC_TILE<D>;
 template <int D>
-constexpr int DEC_SMEM = DEC_WARPS * DEC_STAGES * 2 * DEC_TILE<D> * D;
+constexpr int DEC_STAGES = D == 128 ? 2 : 3;  // tiles in flight per warp
+template <int D>
+constexpr int DEC_SMEM = DEC_WARPS * DEC_STAGES<D> * 2 * DEC_TILE<D> * D;
 
 struct DecodeWork {
     int *counters;  // [grid] arrivals at the pair that starts last in a CTA, zero between launches
@@ -94,16 +95,17 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t u) {
 // PAGED8: block_size is a multiple of 8, so that 8 consecutive positions share a page and its scales;
 // otherwise every position looks its page up for itself.
 template <int D, int G, typename T, bool PAGED8>
-__global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams p, const DecodeWork w) {
-    constexpr int U = 128 / D;          // 16-position MMA rows of a tile
+__global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams p, const DecodeWork w) {
+    constexpr int U = 2;                // 16-position MMA rows of a tile
     constexpr int TILE = DEC_TILE<D>, CHUNK = DEC_CHUNK<D>;
     constexpr int KC = D / 64;          // 16-byte chunks of a K row per thread
     constexpr int VW = D / 32;          // words of a V row per thread
     constexpr int VB = 4 * VW;          // ... bytes
     constexpr int MT = D / 16;          // 16-dim row tiles of O^T
     constexpr int WIN = 16 / U;         // tiles of a window of page look-ups
-    constexpr int STAGES = DEC_STAGES, K_BYTES = TILE * D, STAGE = 2 * K_BYTES;
+    constexpr int STAGES = DEC_STAGES<D>, K_BYTES = TILE * D, STAGE = 2 * K_BYTES;
     constexpr float M_NONE = -1e30f;    // below every score; finite, so that 2^(-inf - M) is 0
+    constexpr float V_LEAST = 5.0487098e-29f;  // 2^-94: a weight is at most 2^6 / V_LEAST, sums of them stay finite
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r0 = lane >> 2, q4 = lane & 3;
     const int64_t table_positions = static_cast<int64_t>(p.bt_cols) * p.block_size;
@@ -111,7 +113,10 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
     extern __shared__ __align__(16) uint8_t s_ring[];  // [DEC_WARPS][STAGES][K, V]; between pairs the warps' sums
     auto s_acc = reinterpret_cast<float (*)[G][D + 4]>(s_ring);
     static_assert(G * (D + 4) * 4 <= STAGES * STAGE, "the sums fit the ring");
-    __shared__ float s_scale[PAGED8 ? 1 : DEC_WARPS][PAGED8 ? 1 : STAGES][PAGED8 ? 1 : TILE][2];
+    // PAGED8: of each group of 8 positions its first row in the pool / 8 (-1: not to be read), K scale,
+    // V scale and max(|V scale|, V_LEAST), for the window of tiles in use and the next one
+    __shared__ float4 s_table[PAGED8 ? DEC_WARPS : 1][2][32];
+    __shared__ float2 s_scale[PAGED8 ? 1 : DEC_WARPS][PAGED8 ? 1 : STAGES][PAGED8 ? 1 : TILE];
     __shared__ float s_ml[DEC_WARPS][G][2];
     __shared__ float s_w[DEC_MAX_SPLITS + 2][G], s_l[G];
     __shared__ int s_scan[DEC_WARPS], s_max[DEC_WARPS];
@@ -125,12 +130,20 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
         return static_cast<int>(min(static_cast<int64_t>(max(c, 0)), table_positions));
     };
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) + warp * STAGES * STAGE;
-    int window = 0;  // of the tile being consumed
-    auto slot_window = [](int i) { return i / WIN; };
-    auto copy_v = [](uint32_t dst, const int8_t *src) {
-        if constexpr (VW == 4) copy16(dst, src);
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    // 16-byte chunk c of 128-byte line i of a slot (a row at D = 128, two at D = 64) is kept at c ^ swizzle(i),
+    // which spreads the operand reads below over all banks.
+    auto k_swizzle = [](int line) { return D == 128 ? (line & 1) << 2 : (line & 3) << 1; };
+    auto v_swizzle = [](int line) { return D == 128 ? ((line >> 1) & 3) << 1 : (line & 3) << 1; };
+    auto place = [](int row, int byte, auto swizzle) {  // offset of a byte of a row in its slot
+        const int line = row * D / 128, at = row * D % 128 + byte;
+        return static_cast<uint32_t>(line * 128 + ((((at >> 4) ^ swizzle(line))) << 4) + (at & 15));
     };
+    // Operand reads of the first 8 rows; every 8 rows the pattern repeats.
+    uint32_t k_off[KC], v_off[2];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) k_off[c] = place(r0, 16 * (q4 + 4 * c), k_swizzle);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) v_off[y] = place(2 * q4 + y, VB * r0, v_swizzle);
     auto lds_v = [](uint32_t (&v)[VW], uint32_t src) {
         if constexpr (VW == 4) {
             const uint4 x = lds16(src);
@@ -272,7 +285,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 
-        // ---- pages: lane 2 U i + g holds those of group g (8 positions) of tile i of a window of this warp's tiles
+        // ---- pages
         const int *table = p.block_table + e * p.bt_stride;
         const int tiles = pos1 > pos0 ? (pos1 - pos0 + TILE - 1) / TILE : 0;
         const int mine = tiles > warp ? (tiles - warp + DEC_WARPS - 1) / DEC_WARPS : 0;  // tiles warp, warp + 4, ...
@@ -293,90 +306,108 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
             k = blk >= 0 ? __ldcg(p.k_scale + cell) : 0.f;
             v = blk >= 0 ? __ldcg(p.v_scale + cell) : 0.f;
         };
+        // Look-ups run three windows ahead of their use: block ids, then scales, then the table.
+        // Here lane 2 U i + g works for group g (8 positions) of tile i of the window.
         auto group_pos = [&](int window) { return tile_pos(window * WIN + lane / (2 * U)) + 8 * (lane % (2 * U)); };
-        // The window being consumed, the next one (its loads in flight) and the block ids of the one after
-        int row_now = -1, row_next = -1, blk_after = -1;  // a group's first row in the pool / 8, -1: nothing to read
-        float k_now = 0.f, v_now = 0.f, k_next = 0.f, v_next = 0.f;
         auto lookup = [&](int window) { return window * WIN + lane / (2 * U) < mine ? page_of(group_pos(window)) : -1; };
-        auto next_window = [&](int window) {  // fills *_next for `window` from blk_after
-            scales(blk_after, k_next, v_next);
+        int blk_pending = -1, blk_scaled = -1;
+        float k_pending = 0.f, v_pending = 0.f;
+        unsigned dead_windows = 0;  // bit (window & 1): it holds pages that are not to be read
+        auto load_scales = [&](int window) {  // of the window whose block ids are pending, and the next one's ids
+            blk_scaled = blk_pending;
+            scales(blk_scaled, k_pending, v_pending);
+            blk_pending = lookup(window + 1);
+        };
+        auto write_table = [&](int window) {
             const int per = p.block_size >> 3;
-            row_next = blk_after < 0 ? -1 : (blk_after * p.H_kv + kvh) * per + (group_pos(window) >> 3) % per;
-            blk_after = lookup(window + 1);
+            const int row8 = blk_scaled < 0 ? -1 : (blk_scaled * p.H_kv + kvh) * per + (group_pos(window) >> 3) % per;
+            s_table[warp][window & 1][lane] = make_float4(__int_as_float(row8), k_pending, v_pending, fmaxf(fabsf(v_pending), V_LEAST));
+            const bool gone = row8 < 0 && window * WIN + lane / (2 * U) < mine && group_pos(window) < pos1;
+            const unsigned bit = 1u << (window & 1);
+            dead_windows = __any_sync(0xffffffffu, gone) ? dead_windows | bit : dead_windows & ~bit;
+            __syncwarp();
         };
 
-        // Copies of tile i into its slot of the ring, thread-private: each thread copies what it will read.
+        // Copies of tile i into its slot of the ring, 512 contiguous bytes of the pool an instruction: a
+        // quarter of the warp fills one 128-byte line, chunk c of it at position c ^ swizzle.
         auto issue = [&](int i, int slot) {
-            const uint32_t dst = ring + slot * STAGE;
+            const uint32_t dst = ring + slot * STAGE + (lane >> 3) * 128;
             if (i < mine) {
-                const int pos = tile_pos(i);
-                [[maybe_unused]] int row = 0;
-                if constexpr (!PAGED8) {  // lane j: position pos + j, its scales kept beside the ring
+                if constexpr (PAGED8) {
+#pragma unroll
+                    for (int g = 0; g < 2 * U; ++g) {
+                        const int row8 = max(__float_as_int(s_table[warp][(i / WIN) & 1][(i % WIN) * 2 * U + g].x), 0);
+                        const int64_t base = static_cast<int64_t>(row8) * (8 * D) + lane * 16;
+#pragma unroll
+                        for (int x = 0; x < D / 64; ++x) {
+                            const int line = (g * (D / 64) + x) * 4;
+                            copy16(dst + line * 128 + (((lane & 7) ^ k_swizzle(line + (lane >> 3))) << 4), p.k_pool + base + 512 * x);
+                            copy16(dst + K_BYTES + line * 128 + (((lane & 7) ^ v_swizzle(line + (lane >> 3))) << 4),
+                                   p.v_pool + base + 512 * x);
+                        }
+                    }
+                } else {  // lane j: position pos + j, its scales kept beside the ring
+                    const int pos = tile_pos(i);
                     const int blk = lane < TILE ? page_of(pos + lane) : -1;
                     float ks, vs;
                     scales(blk, ks, vs);
-                    if (lane < TILE) {
-                        s_scale[warp][slot][lane][0] = blk < 0 ? -INFINITY : ks;  // -inf: not to be read
-                        s_scale[warp][slot][lane][1] = vs;
-                    }
-                    row = max(blk, 0);
-                    __syncwarp();
-                }
+                    if (lane < TILE) s_scale[warp][slot][lane] = make_float2(blk < 0 ? -INFINITY : ks, vs);  // -inf: not to be read
+                    const int row = max(blk, 0);
 #pragma unroll
-                for (int g = 0; g < 2 * U; ++g) {
-                    if constexpr (PAGED8) {
-                        const bool ahead = slot_window(i) != window;
-                        const int src = (i % WIN) * 2 * U + g;
-                        const int row8 = max(__shfl_sync(0xffffffffu, ahead ? row_next : row_now, src), 0);
-                        const int64_t base = static_cast<int64_t>(row8) * (8 * D);
-#pragma unroll
-                        for (int c = 0; c < KC; ++c)
-                            copy16(dst + (g * KC + c) * 512 + lane * 16, p.k_pool + base + r0 * D + 16 * (q4 + 4 * c));
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-                            copy_v(dst + K_BYTES + (2 * g + y) * (32 * VB) + lane * VB, p.v_pool + base + (2 * q4 + y) * D + VB * r0);
-                    } else {
-                        auto at_row = [&](int j) {
-                            const int64_t cell = static_cast<int64_t>(__shfl_sync(0xffffffffu, row, j)) * p.H_kv + kvh;
-                            return (cell * p.block_size + (pos + j) % p.block_size) * D;
-                        };
-                        const int64_t kb = at_row(8 * g + r0);
-#pragma unroll
-                        for (int c = 0; c < KC; ++c)
-                            copy16(dst + (g * KC + c) * 512 + lane * 16, p.k_pool + kb + 16 * (q4 + 4 * c));
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-                            copy_v(dst + K_BYTES + (2 * g + y) * (32 * VB) + lane * VB, p.v_pool + at_row(8 * g + 2 * q4 + y) + VB * r0);
+                    for (int line = 0; line < TILE * D / 128; line += 4) {
+                        const int byte = (line + (lane >> 3)) * 128 + (lane & 7) * 16, j = byte / D;
+                        const int64_t cell = static_cast<int64_t>(__shfl_sync(0xffffffffu, row, j)) * p.H_kv + kvh;
+                        const int64_t base = (cell * p.block_size + (pos + j) % p.block_size) * D + byte % D;
+                        copy16(dst + line * 128 + (((lane & 7) ^ k_swizzle(line + (lane >> 3))) << 4), p.k_pool + base);
+                        copy16(dst + K_BYTES + line * 128 + (((lane & 7) ^ v_swizzle(line + (lane >> 3))) << 4), p.v_pool + base);
                     }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 
-        window = 0;
         if constexpr (PAGED8) {
-            blk_after = lookup(0);
-            next_window(0);
-            row_now = row_next;
-            k_now = k_next;
-            v_now = v_next;
-            next_window(1);
+            blk_pending = lookup(0);
+            load_scales(0);
+            write_table(0);
+            load_scales(1);
         }
         for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
         int slot = 0;
         for (int i = 0; i < mine; ++i) {
             if constexpr (PAGED8) {
-                if (i % WIN == 0 && i > 0) {
-                    ++window;
-                    row_now = row_next;
-                    k_now = k_next;
-                    v_now = v_next;
-                    next_window(window + 1);
+                if (i % WIN == 0) {  // entering a window: the next one's table, whose rows the copies are about to need
+                    write_table(i / WIN + 1);
+                    load_scales(i / WIN + 2);
                 }
             }
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();  // every lane's copies of this tile have landed, the previous tile's slot is free
             issue(i + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
             const uint32_t src = ring + slot * STAGE;
+            float ck[U][2][2], sv[U][2], sc[U][2];  // score factors of the two heads, V scale, |V scale| bounded below
+            bool gone[U][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float k;
+                    if constexpr (PAGED8) {
+                        const float4 t = s_table[warp][(i / WIN) & 1][(i % WIN) * 2 * U + 2 * u + h];
+                        gone[u][h] = __float_as_int(t.x) < 0;
+                        k = t.y;
+                        sv[u][h] = t.z;
+                        sc[u][h] = t.w;
+                    } else {
+                        const float2 t = s_scale[warp][slot][16 * u + 8 * h + r0];
+                        gone[u][h] = t.x == -INFINITY;
+                        k = t.x;
+                        sv[u][h] = t.y;
+                        sc[u][h] = fmaxf(fabsf(t.y), V_LEAST);
+                    }
+                    ck[u][h][0] = c0 * k;
+                    ck[u][h][1] = c1 * k;
+                }
             // ---- S^T = K Q^T -------------------------------------------------------------
             float s[U][4];
 #pragma unroll
@@ -385,8 +416,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
                 s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
-                    const uint4 ka = lds16(src + (2 * u * KC + c) * 512 + lane * 16);
-                    const uint4 kb = lds16(src + ((2 * u + 1) * KC + c) * 512 + lane * 16);
+                    const uint4 ka = lds16(src + (16 * u) * D + k_off[c]);  // rows r0 and r0 + 8, chunk q4 + 4 c
+                    const uint4 kb = lds16(src + (16 * u + 8) * D + k_off[c]);
                     const uint32_t a[4] = {ka.x, ka.y, ka.z, ka.w}, b[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -398,50 +429,40 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[u][j] += odd[j];
             }
-            // ---- scores in base 2, masks --------------------------------------------------
+            // ---- weights 2^(t - M) --------------------------------------------------------
             const int pos = tile_pos(i);
-            float sv[U][2];
-            bool dead = false;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float sk;
-                    bool gone;
-                    if constexpr (PAGED8) {
-                        const int lane_of = (i % WIN) * 2 * U + 2 * u + h;
-                        sk = __shfl_sync(0xffffffffu, k_now, lane_of);
-                        sv[u][h] = __shfl_sync(0xffffffffu, v_now, lane_of);
-                        gone = __shfl_sync(0xffffffffu, row_now, lane_of) < 0;
-                    } else {
-                        sk = s_scale[warp][slot][16 * u + 8 * h + r0][0];
-                        sv[u][h] = s_scale[warp][slot][16 * u + 8 * h + r0][1];
-                        gone = sk == -INFINITY;
-                    }
-                    s[u][2 * h] *= c0 * sk;
-                    s[u][2 * h + 1] *= c1 * sk;
-                    if (gone) s[u][2 * h] = s[u][2 * h + 1] = -INFINITY;
-                    dead |= gone;
-                }
-            const bool masks = pos + TILE > pos1 || __any_sync(0xffffffffu, dead);
+            const bool masks = pos + TILE > pos1 || (PAGED8 ? (dead_windows >> ((i / WIN) & 1)) & 1u : true);
             if (masks) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (pos + 16 * u + 8 * h + r0 >= pos1) s[u][2 * h] = s[u][2 * h + 1] = -INFINITY;
+                    for (int h = 0; h < 2; ++h) gone[u][h] |= pos + 16 * u + 8 * h + r0 >= pos1;
             }
-            // ---- does anything exceed M by 2^6? -------------------------------------------
-            float x0 = -INFINITY, x1 = -INFINITY;
+            float wt[U][4], most = 0.f;  // most: the largest weight as it would enter the sum over V
+            auto weigh = [&] {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float lv = __log2f(fmaxf(fabsf(sv[u][h]), 7.8886e-31f));  // 2^-100: p stays below 2^106
-                    x0 = fmaxf(x0, s[u][2 * h] + lv);
-                    x1 = fmaxf(x1, s[u][2 * h + 1] + lv);
-                }
-            if (__any_sync(0xffffffffu, x0 > m0 + 6.f || x1 > m1 + 6.f)) {
+                    for (int h = 0; h < 2; ++h) {
+                        wt[u][2 * h] = ex2_approx(fmaf(s[u][2 * h], ck[u][h][0], -m0));
+                        wt[u][2 * h + 1] = ex2_approx(fmaf(s[u][2 * h + 1], ck[u][h][1], -m1));
+                        if (masks && gone[u][h]) wt[u][2 * h] = wt[u][2 * h + 1] = 0.f;
+                        most = fmaxf(most, fmaxf(wt[u][2 * h], wt[u][2 * h + 1]) * sc[u][h]);
+                    }
+            };
+            weigh();
+            if (__any_sync(0xffffffffu, most > 64.f)) {  // M has to move
+                float x0 = M_NONE, x1 = M_NONE;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float lv = __log2f(sc[u][h]);
+                        if (!(masks && gone[u][h])) {
+                            x0 = fmaxf(x0, fmaf(s[u][2 * h], ck[u][h][0], lv));
+                            x1 = fmaxf(x1, fmaf(s[u][2 * h + 1], ck[u][h][1], lv));
+                        }
+                    }
 #pragma unroll
                 for (int k = 4; k < 32; k <<= 1) {
                     x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, k));
@@ -460,19 +481,18 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
                     acc[t][2] *= f0;
                     acc[t][3] *= f1;
                 }
+                weigh();
             }
-            // ---- weights, and P^T as the column operand ------------------------------------
+            // ---- P^T as the column operand -------------------------------------------------
             uint32_t pb[U][2];
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float w0 = ex2_approx(s[u][2 * h] - m0), w1 = ex2_approx(s[u][2 * h + 1] - m1);
-                    l0 += w0;
-                    l1 += w1;
-                    // a masked position has weight 0, whatever its page's scale
-                    float y0 = w0 * sv[u][h], y1 = w1 * sv[u][h];
-                    if (masks && s[u][2 * h] == -INFINITY) y0 = y1 = 0.f;
+                    l0 += wt[u][2 * h];
+                    l1 += wt[u][2 * h + 1];
+                    float y0 = wt[u][2 * h] * sv[u][h], y1 = wt[u][2 * h + 1] * sv[u][h];
+                    if (masks && gone[u][h]) y0 = y1 = 0.f;  // whatever its page's scale
                     pb[u][h] = movm_trans(half2_of(y0, y1));
                 }
             // ---- O^T += V^T P^T -------------------------------------------------------------
@@ -480,7 +500,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
             for (int u = 0; u < U; ++u) {
                 uint32_t v[4][VW];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) lds_v(v[y], src + K_BYTES + (4 * u + y) * (32 * VB) + lane * VB);
+                for (int y = 0; y < 4; ++y) lds_v(v[y], src + K_BYTES + (16 * u + 8 * (y >> 1)) * D + v_off[y & 1]);
 #pragma unroll
                 for (int x = 0; x < VW; ++x) {
                     const uint32_t a = v[0][x] ^ 0x80808080u, b = v[1][x] ^ 0x80808080u;
@@ -492,7 +512,6 @@ __global__ void __launch_bounds__(DEC_THREADS, 4) decode_kernel(const AttnParams
                 }
             }
             slot = slot + 1 == STAGES ? 0 : slot + 1;
-            if constexpr (!PAGED8) __syncwarp();  // the slot's scales are free for the next tile's
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
