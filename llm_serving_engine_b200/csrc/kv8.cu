@@ -10,6 +10,7 @@
 #include "kv8_append.cuh"
 #include "kv8_attn.cuh"
 #include "kv8_decode.cuh"
+#include "kv8_prompt.cuh"
 
 namespace lse {
 
@@ -19,6 +20,8 @@ cudaError_t kv8_device_status(int *status, bool reset) {
     if (e == cudaSuccess && reset) e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
     return e;
 }
+
+cudaError_t kv8_set_wait_limit(long long cycles) { return cudaMemcpyToSymbol(g_wait_limit, &cycles, sizeof(cycles)); }
 
 namespace {
 
@@ -32,7 +35,7 @@ int check_cache(int64_t H, int64_t H_kv, int64_t D, const void *k_pool, const vo
     const int64_t G = H / H_kv;
     if ((D != 64 && D != 128) || (G != 1 && G != 2 && G != 4 && G != 8)) return LSE_ERR_UNSUPPORTED;
     if (H > 65535 || block_size > 65536 || num_blocks > INT32_MAX / 2 || num_blocks * block_size > INT32_MAX / 2 ||
-        num_blocks * block_size / 8 * H_kv > INT32_MAX)
+        num_blocks * block_size > UINT32_MAX / H_kv)  // rows of a pool are counted in 32 bits
         return LSE_ERR_UNSUPPORTED;
     if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
         return LSE_ERR_ALIGNMENT;
@@ -101,15 +104,6 @@ int run_append(const void *qkv, int64_t M, int64_t ld_qkv, int64_t H, int64_t H_
     return launch_append(p, sms, st);
 }
 
-template <int D, typename T>
-int launch_rows(const kv8::AttnParams &p, int sms, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    const int64_t blocks = std::min<int64_t>((static_cast<int64_t>(p.tokens) * p.H + 7) / 8, 64LL * sms);
-    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st);
-    return finish(cudaLaunchKernelEx(&cfg, kv8::attn_rows_kernel<D, T>, p), "kv8 attention launch");
-}
-
 // Resident CTAs per SM of the decode kernel (its launch bounds) and so the launch's grid.
 constexpr int kDecodePerSm = 3;
 
@@ -137,9 +131,23 @@ int launch_decode_g(int64_t G, const kv8::AttnParams &p, const kv8::DecodeWork &
     }
 }
 
-int launch_attention(const kv8::AttnParams &p, int dtype, int64_t D, int sms, cudaStream_t st) {
-    if (dtype == LSE_F16) return D == 128 ? launch_rows<128, __half>(p, sms, st) : launch_rows<64, __half>(p, sms, st);
-    return D == 128 ? launch_rows<128, __nv_bfloat16>(p, sms, st) : launch_rows<64, __nv_bfloat16>(p, sms, st);
+size_t prompt_counter_bytes(int sms) { return (static_cast<size_t>(sms) * sizeof(int) + 255) / 256 * 256; }
+
+template <int D, typename T>
+int launch_prompt(const kv8::AttnParams &p, void *workspace, int sms, cudaStream_t st) {
+    kv8::PromptWork w{};
+    w.counters = static_cast<int *>(workspace);
+    w.acc = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + prompt_counter_bytes(sms));
+    w.ml = w.acc + 2ll * sms * kv8::PR_ROWS * D;
+    constexpr int smem = kv8::PromptSmem<D>::BYTES;
+    cudaError_t e = cudaFuncSetAttribute(kv8::prompt_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return finish(e, "kv8_paged_attention attributes");
+    int log_g = 0;
+    while ((1 << log_g) < p.H / p.H_kv) ++log_g;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(sms)), dim3(kv8::PR_THREADS), smem, st);
+    return finish(cudaLaunchKernelEx(&cfg, kv8::prompt_kernel<D, T>, p, w, log_g), "kv8_paged_attention launch");
 }
 
 }  // namespace
@@ -264,10 +272,10 @@ int lse_kv8_decode_attention(const void *q, int dtype, int64_t E, int64_t H, int
 }
 
 size_t lse_kv8_paged_attention_workspace(int64_t H, int64_t H_kv, int64_t D) {
-    (void)H;
-    (void)H_kv;
-    (void)D;
-    return 0;
+    int dev = 0;
+    if (H <= 0 || H_kv <= 0 || D <= 0 || H % H_kv || host::current_device(&dev)) return 0;
+    const int sms = host::num_sms(dev);
+    return prompt_counter_bytes(sms) + 2ull * sms * kv8::PR_ROWS * (D + 2) * sizeof(float);
 }
 
 int lse_kv8_paged_attention(const void *q, int dtype, int64_t tokens, int64_t H, int64_t D, int64_t q_stride_h,
@@ -277,8 +285,6 @@ int lse_kv8_paged_attention(const void *q, int dtype, int64_t tokens, int64_t H,
                             const int32_t *query_offset, const int32_t *q_start, const int32_t *q_len, int64_t E,
                             float scale, void *o, int64_t o_stride_h, int64_t o_stride_m, void *workspace,
                             size_t workspace_bytes, void *stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     if (E < 0 || tokens < 0) return LSE_ERR_INVALID_ARG;
     if (dtype != LSE_BF16 && dtype != LSE_F16) return LSE_ERR_UNSUPPORTED;
     if (E == 0 || tokens == 0) return LSE_OK;
@@ -317,7 +323,12 @@ int lse_kv8_paged_attention(const void *q, int dtype, int64_t tokens, int64_t H,
     p.block_size = static_cast<int>(block_size);
     p.num_blocks = static_cast<int>(num_blocks);
     p.scale_log2 = scale * 1.4426950408889634f;
-    return launch_attention(p, dtype, D, host::num_sms(dev), static_cast<cudaStream_t>(stream));
+    if (!workspace || workspace_bytes < lse_kv8_paged_attention_workspace(H, H_kv, D)) return LSE_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return LSE_ERR_ALIGNMENT;
+    const int sms = host::num_sms(dev);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == LSE_F16) return D == 128 ? launch_prompt<128, __half>(p, workspace, sms, st) : launch_prompt<64, __half>(p, workspace, sms, st);
+    return D == 128 ? launch_prompt<128, __nv_bfloat16>(p, workspace, sms, st) : launch_prompt<64, __nv_bfloat16>(p, workspace, sms, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,771 @@
+// Attention of any number of query tokens per entry (prompts, prompt chunks, mixed batches) over the
+// 8-bit paged K/V cache, on the 5th-generation tensor cores:
+//
+//   o[h, t, :] = sum_p w_p v_scale[b_p] v_code[p, :] / sum_p w_p,   w_p = 2^(t_p),
+//   t_p = scale log2(e) k_scale[b_p] (q[h, t, :] . k_code[p, :]),   p < limit(t)
+//
+// One CTA per SM works on 256 rows (the G query heads of 256 / G consecutive tokens, which share a
+// KV head) as two tiles of 128, 128 positions at a time:
+//   * four converter warps read the codes of a position tile (16-byte loads, one tile ahead in
+//     registers), turn them into fp16, exact, and lay K (K-major) and V (as it lies, MN-major) out in
+//     shared memory with the 128-byte swizzle, two tiles each;
+//   * one thread issues tcgen05.mma: S = Q K^T for both tiles, and O += P V with P from tensor
+//     memory, in the order PV_a(j), QK_a(j + 1), PV_b(j), QK_b(j + 1): while one tile's softmax runs the
+//     tensor core has the other tile's products;
+//   * four softmax warps per tile, one row a thread: S comes from tensor memory 32 positions at a
+//     time, the weights go back over it as fp16.  The page scales multiply scores and weights
+//     (from a table in shared memory), so the products themselves are of integers and q.  M >=
+//     max(t_p + log2 v_scale) - 6 moves only when a weight exceeds 2^6, and with it the row of O.
+// Tensor memory: S_a | S_b | O_a | O_b, 128 columns each.
+//
+// The work, (entry, KV head, 256-row item) x position tiles laid end to end, is cut into equal runs
+// of tiles, one per SM, from the lengths on the device; items that several CTAs share are joined by the
+// last to arrive, in the order of the positions.  Where items are short (fewer than SPLIT_TILES tiles on
+// average) they are dealt whole instead: a joint costs more than it gains there.
+#pragma once
+
+#include "common.cuh"
+#include "kv8_attn.cuh"
+#include "kv8_decode.cuh"
+#include "tc_ptx.cuh"
+
+namespace lse {
+namespace kv8 {
+
+constexpr int PR_ROWS = 256;        // rows of an item
+constexpr int PR_KEYS = 128;        // positions of a tile
+constexpr int PR_CONVERT = 8;       // first converter warp (after the 2 x 4 softmax warps)
+constexpr int PR_MMA = 12;          // the MMA warp
+constexpr int PR_WARPS = 13;
+constexpr int PR_THREADS = PR_WARPS * 32;
+constexpr int PR_TABLES = 4;        // scale tables in flight
+constexpr int PR_SPLIT_TILES = 8;
+
+struct PromptWork {
+    int *counters;  // [grid], as DecodeWork
+    float *acc;     // [2 * grid][2][D / 4][128][4] partial sums, row-contiguous float4s
+    float *ml;      // [2 * grid][256][2]
+};
+
+template <int D>
+struct PromptSmem {
+    static constexpr int TILE = PR_KEYS * D * 2;  // fp16 K or V tile; a Q tile is the same
+    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, TABLE = V + 2 * TILE;
+    static constexpr int BYTES = TABLE + PR_TABLES * (PR_KEYS * 8 + 32) + 1024;  // + alignment
+};
+
+// What a CTA does next: position tiles [j0, j1) of item i of (entry e, KV head kvh).
+struct PromptSegment {
+    int e, kvh, i, j0, j1, tiles;
+    int q_start, q_len, offset, context;
+};
+
+// The schedule, the same in every role; see the header comment.
+struct PromptSchedule {
+    const AttnParams *p;
+    int tok;            // tokens per item
+    int64_t at, end, total, active;  // split: this CTA's run of tiles; whole: its next item and their number
+    bool split;
+    int e, kvh, i;
+    int64_t first;      // split: first tile of the current item; whole: first item of entry e
+    int q_start, q_len, offset, context, nq;
+
+    __device__ __forceinline__ static int context_of(const AttnParams &p, int e) {
+        const int64_t most = static_cast<int64_t>(p.bt_cols) * p.block_size;
+        return static_cast<int>(min(static_cast<int64_t>(max(__ldcg(p.context_len + e), 0)), most));
+    }
+    __device__ __forceinline__ static int tiles_of(int context, int offset, int q_len, int tok, int i) {
+        const int64_t seen = min(static_cast<int64_t>(context), static_cast<int64_t>(offset) + min(q_len, (i + 1) * tok));
+        return static_cast<int>(max(static_cast<int64_t>(1), (seen + PR_KEYS - 1) / PR_KEYS));
+    }
+    __device__ __forceinline__ void load_entry() {
+        if (e >= p->E) return;
+        q_start = __ldcg(p->q_start + e);
+        q_len = max(__ldcg(p->q_len + e), 0);
+        offset = __ldcg(p->query_offset + e);
+        context = context_of(*p, e);
+        nq = (q_len + tok - 1) / tok;
+    }
+    __device__ __forceinline__ bool next(PromptSegment &s) {
+        if (at >= end) return false;
+        if (split) {
+            const int n = tiles_of(context, offset, q_len, tok, i);
+            s.j0 = static_cast<int>(at - first);
+            s.j1 = static_cast<int>(min(end, first + n) - first);
+            fill(s, n);
+            at = first + s.j1;
+            if (s.j1 == n) {  // the next item
+                first += n;
+                if (++i == nq) {
+                    i = 0;
+                    if (++kvh == p->H_kv) {
+                        kvh = 0;
+                        do {
+                            ++e;
+                            load_entry();
+                        } while (e < p->E && nq == 0);
+                    }
+                }
+            }
+        } else {
+            while (at >= first + static_cast<int64_t>(nq) * p->H_kv) {
+                first += static_cast<int64_t>(nq) * p->H_kv;
+                ++e;
+                load_entry();
+            }
+            const int k = static_cast<int>(at - first);
+            kvh = k % p->H_kv;
+            i = nq - 1 - k / p->H_kv;  // the longest first
+            s.j0 = 0;
+            s.j1 = tiles_of(context, offset, q_len, tok, i);
+            fill(s, s.j1);
+            at += active;
+        }
+        return true;
+    }
+    __device__ __forceinline__ void fill(PromptSegment &s, int n) const {
+        s.e = e;
+        s.kvh = kvh;
+        s.i = i;
+        s.tiles = n;
+        s.q_start = q_start;
+        s.q_len = q_len;
+        s.offset = offset;
+        s.context = context;
+    }
+    // CTA whose run holds a tile (split)
+    __device__ __forceinline__ int cta_of(int64_t tile) const { return static_cast<int>(((tile + 1) * active - 1) / total); }
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr)
+        : "memory");
+}
+// Shared-memory descriptor of an MN-major operand with the 128-byte swizzle: rows of 64 elements (128
+// bytes) along the contraction, 8 rows 1024 bytes; `lead` bytes to the next 64 elements of the other index.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t lead) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((lead >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t out2(float lo, float hi) {  // two elements of T in a word
+    if constexpr (std::is_same_v<T, __half>) return half2_of(lo, hi);
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptWork work, const int log_g) {
+    using S = PromptSmem<D>;
+    constexpr float M_NONE = -1e30f, V_LEAST = 5.0487098e-29f;  // as in the decode kernel
+    constexpr int KC = D / 64;                    // 64-dim halves of a row
+    constexpr uint32_t O_COL = 256;               // tensor-memory columns: S 0, 128; O 256, 384
+    // fp16 x fp16 -> fp32, M = 128; S: N = 128 positions, K-major; O: N = D, B MN-major
+    constexpr uint32_t ID_S = (1u << 4) | ((PR_KEYS >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((128u >> 4) << 24);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    enum { K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, S_FULL = 8, P_FULL = 10, Q_FULL = 12, O_FULL = 14, TABLE_FULL = 16,
+           JOIN = TABLE_FULL + PR_TABLES, ROWS, DRAIN, DONE, BARS };
+    extern __shared__ uint8_t s_raw[];
+    __shared__ __align__(8) uint64_t s_bar[BARS];
+    __shared__ uint32_t s_tmem, s_rows[2][PR_KEYS];
+    __shared__ int s_abort_word, s_last;
+    __shared__ int64_t s_sum[PR_WARPS][2];
+    __shared__ int64_t s_found[3];
+    const uint32_t base = (ptx::smem_u32(s_raw) + 1023u) & ~1023u;
+    uint8_t *const s_base = s_raw + (base - ptx::smem_u32(s_raw));
+    volatile int *s_abort = &s_abort_word;
+    auto bar = [&](int i) { return ptx::smem_u32(s_bar) + 8 * i; };
+    auto table_of = [&](int n) { return reinterpret_cast<float *>(s_base + S::TABLE + (n % PR_TABLES) * (PR_KEYS * 8 + 32)); };
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(bar(K_FULL + i), 4);
+            ptx::mbar_init(bar(K_EMPTY + i), 1);
+            ptx::mbar_init(bar(V_FULL + i), 4);
+            ptx::mbar_init(bar(V_EMPTY + i), 1);
+            ptx::mbar_init(bar(S_FULL + i), 1);
+            ptx::mbar_init(bar(P_FULL + i), 4);
+            ptx::mbar_init(bar(Q_FULL + i), 4);
+            ptx::mbar_init(bar(O_FULL + i), 1);
+        }
+        for (int i = 0; i < PR_TABLES; ++i) ptx::mbar_init(bar(TABLE_FULL + i), 4);
+        ptx::mbar_init(bar(JOIN), 8);
+        ptx::mbar_init(bar(ROWS), 4);
+        ptx::mbar_init(bar(DRAIN), 1);
+        ptx::mbar_init(bar(DONE), PR_WARPS);
+        ptx::fence_mbar_init();
+        s_abort_word = 0;
+    }
+    if (warp == PR_MMA) {
+        ptx::tmem_alloc(ptx::smem_u32(&s_tmem), 512);
+        ptx::tmem_relinquish();
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the cache and the lengths come from earlier kernels
+
+    // A barrier of some warps that, unlike bar.sync, gives up with the CTA: every warp arrives once a phase.
+    auto group_sync = [&](int b, int phase) {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(b));
+        const bool ok = ptx::mbar_wait(bar(b), phase & 1, s_abort);
+        return static_cast<bool>(__all_sync(0xffffffffu, ok));
+    };
+
+    // ---- the schedule ------------------------------------------------------------------------------
+    PromptSchedule sched;
+    sched.p = &p;
+    sched.tok = PR_ROWS >> log_g;
+    {
+        auto entry = [&](int e, int64_t &tiles, int64_t &items) {
+            tiles = items = 0;
+            if (e >= p.E) return;
+            const int len = max(__ldcg(p.q_len + e), 0), off = __ldcg(p.query_offset + e);
+            const int ctx = PromptSchedule::context_of(p, e);
+            items = (len + sched.tok - 1) / sched.tok;
+            for (int i = 0; i < items; ++i) tiles += PromptSchedule::tiles_of(ctx, off, len, sched.tok, i);
+        };
+        int64_t tiles_all = 0, items_all = 0;
+        for (int e0 = 0; e0 < p.E; e0 += PR_THREADS) {
+            int64_t tiles, items;
+            const int e = e0 + threadIdx.x;
+            entry(e, tiles, items);
+            if (blockIdx.x == 0 && e < p.E && items > 0) {
+                const int start = __ldcg(p.q_start + e), len = __ldcg(p.q_len + e);
+                const int64_t seen = min(static_cast<int64_t>(__ldcg(p.context_len + e)), static_cast<int64_t>(__ldcg(p.query_offset + e)) + len);
+                if (start < 0 || start > p.tokens - len || seen > static_cast<int64_t>(p.bt_cols) * p.block_size)
+                    report_status(LSE_ERR_INVALID_ARG);
+            }
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) {
+                tiles += __shfl_xor_sync(0xffffffffu, tiles, k);
+                items += __shfl_xor_sync(0xffffffffu, items, k);
+            }
+            if (lane == 0) {
+                s_sum[warp][0] = tiles;
+                s_sum[warp][1] = items;
+            }
+            __syncthreads();
+            for (int i = 0; i < PR_WARPS; ++i) {
+                tiles_all += s_sum[i][0];
+                items_all += s_sum[i][1];
+            }
+            __syncthreads();
+        }
+        tiles_all *= p.H_kv;
+        items_all *= p.H_kv;
+        sched.split = tiles_all >= PR_SPLIT_TILES * items_all;
+        sched.total = tiles_all;
+        sched.e = -1;
+        sched.kvh = sched.i = 0;
+        sched.first = 0;
+        sched.nq = 0;
+        if (sched.split) {
+            // no run shorter than SPLIT_TILES tiles
+            sched.active = max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), tiles_all / PR_SPLIT_TILES));
+            const bool in = static_cast<int64_t>(blockIdx.x) < sched.active;
+            sched.at = in ? blockIdx.x * tiles_all / sched.active : 0;
+            sched.end = in ? (blockIdx.x + 1) * tiles_all / sched.active : 0;
+            // the entry that tile `at` belongs to
+            if (threadIdx.x == 0) s_found[0] = -1;
+            int64_t before_all = 0;
+            for (int e0 = 0; e0 < p.E; e0 += PR_THREADS) {
+                int64_t tiles, items;
+                entry(e0 + threadIdx.x, tiles, items);
+                int64_t incl = tiles;
+#pragma unroll
+                for (int k = 1; k < 32; k <<= 1) {
+                    const int64_t v = __shfl_up_sync(0xffffffffu, incl, k);
+                    if (lane >= k) incl += v;
+                }
+                if (lane == 31) s_sum[warp][0] = incl;
+                __syncthreads();
+                int64_t before = before_all + incl - tiles;
+                for (int i = 0; i < PR_WARPS; ++i) {
+                    if (i < warp) before += s_sum[i][0];
+                    before_all += s_sum[i][0];
+                }
+                if (tiles > 0 && sched.at >= before * p.H_kv && sched.at < (before + tiles) * p.H_kv) {
+                    s_found[0] = e0 + threadIdx.x;
+                    s_found[1] = before * p.H_kv;
+                    s_found[2] = tiles;
+                }
+                __syncthreads();
+            }
+            if (sched.at < sched.end) {
+                sched.e = static_cast<int>(s_found[0]);
+                sched.load_entry();
+                const int64_t off = sched.at - s_found[1];
+                sched.kvh = static_cast<int>(off / s_found[2]);
+                sched.first = s_found[1] + sched.kvh * s_found[2];
+                for (int n; sched.first + (n = PromptSchedule::tiles_of(sched.context, sched.offset, sched.q_len, sched.tok, sched.i)) <= sched.at; ++sched.i)
+                    sched.first += n;
+            }
+        } else {
+            sched.active = gridDim.x;
+            sched.at = blockIdx.x;
+            sched.end = items_all;
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&s_tmem);
+
+    if (warp < PR_CONVERT) {
+        // ==== softmax: one row a thread =============================================================
+        const int t = warp >> 2;                       // tile a or b
+        const int row = threadIdx.x & 127;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // tensor-memory lane offset of this warp
+        const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + O_COL + 128 * t;
+        uint8_t *const q_tile = s_base + S::Q + t * S::TILE;
+        int n = 0, seg_n = 0, joins = 0;  // position tiles, segments and joint barriers so far
+        PromptSegment s;
+        float back = 1.f;
+        // Writes this row of Q as fp16 (scaled to [1, 2) at its largest by a power of two for bf16).
+        auto write_q = [&](const PromptSegment &x) {
+            const int r = 128 * t + row, in = x.i * sched.tok + (r >> log_g), tok = x.q_start + in;
+            const bool live = in < x.q_len && tok >= 0 && tok < p.tokens;
+            const T *src = static_cast<const T *>(p.q) + tok * p.q_st + static_cast<int64_t>((x.kvh << log_g) + (r & ((1 << log_g) - 1))) * p.q_sh;
+            float down = 1.f;
+            back = 1.f;
+            if constexpr (!std::is_same_v<T, __half>) {
+                float top = 0.f;
+                if (live)
+#pragma unroll
+                    for (int c = 0; c < D / 8; ++c) {
+                        const uint4 v = reinterpret_cast<const uint4 *>(src)[c];
+                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 f = bf16x2_to_f32x2(u[k]);
+                            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                        }
+                    }
+                int k = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+                k = top > 0.f && k < 128 ? max(-120, min(k, 120)) : 0;
+                down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+                back = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+            }
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (live) v = reinterpret_cast<const uint4 *>(src)[c];
+                if constexpr (!std::is_same_v<T, __half>) {
+                    uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = bf16x2_to_f32x2(u[k]);
+                        u[k] = half2_of(f.x * down, f.y * down);
+                    }
+                    v = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+                *reinterpret_cast<uint4 *>(q_tile + (c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(Q_FULL + t));
+        };
+        bool ok = true;
+        bool more = sched.next(s);
+        if (more) write_q(s);
+        while (more && ok) {
+            const int r = 128 * t + row, in = s.i * sched.tok + (r >> log_g);
+            const int tok = s.q_start + in;
+            const bool live = in < s.q_len && tok >= 0 && tok < p.tokens;
+            const int limit = live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(s.context), static_cast<int64_t>(s.offset) + in + 1))) : 0;
+            const bool warp_live = __any_sync(0xffffffffu, live);
+            const float c = p.scale_log2 * back;
+            float M = M_NONE;
+            float2 l2 = make_float2(0.f, 0.f);
+            for (int j = s.j0; j < s.j1; ++j, ++n) {
+                ok = ptx::mbar_wait(bar(TABLE_FULL + n % PR_TABLES), (n / PR_TABLES) & 1, s_abort) && ptx::mbar_wait(bar(S_FULL + t), n & 1, s_abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                if (!warp_live) {  // no row of this warp is stored: its weights do not matter
+                    if (lane == 0) ptx::mbar_arrive(bar(P_FULL + t));
+                    continue;
+                }
+                const float *table = table_of(n);
+                const uint32_t *bits = reinterpret_cast<const uint32_t *>(table + 2 * PR_KEYS);  // 4 words dead, 4 words mute
+                const int pos = j * PR_KEYS;
+#pragma unroll 1
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint32_t sr[32];
+                    ptx::tmem_ld_32x32b_x32(s_col + 32 * ch, sr);
+                    const uint32_t dead = bits[ch], mute = bits[4 + ch];
+                    const int left = limit - pos - 32 * ch;
+                    const uint32_t seen = (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u) & ~dead;
+                    const bool masks = __any_sync(0xffffffffu, (seen & ~mute) != ~0u);
+                    const float4 *sk = reinterpret_cast<const float4 *>(table + 32 * ch), *sv = reinterpret_cast<const float4 *>(table + PR_KEYS + 32 * ch);
+                    ptx::tmem_wait_ld();
+                    uint32_t pk[16];
+                    float most;
+                    float2 add;
+                    auto weigh = [&](auto masked) {
+                        most = 0.f;
+                        add = make_float2(0.f, 0.f);
+                        const float2 c2 = make_float2(c, c), m2 = make_float2(-M, -M);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 a = sk[k], b = sv[k];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float2 x = make_float2(__uint_as_float(sr[4 * k + 2 * h]), __uint_as_float(sr[4 * k + 2 * h + 1]));
+                                float2 w = __ffma2_rn(__fmul2_rn(x, h ? make_float2(a.z, a.w) : make_float2(a.x, a.y)), c2, m2);
+                                w.x = ex2_approx(w.x);
+                                w.y = ex2_approx(w.y);
+                                const float2 v = h ? make_float2(b.z, b.w) : make_float2(b.x, b.y);
+                                float2 y = __fmul2_rn(w, v);
+                                if constexpr (decltype(masked)::value) {
+                                    if (!((seen >> (4 * k + 2 * h)) & 1u)) w.x = 0.f;
+                                    if (!((seen >> (4 * k + 2 * h + 1)) & 1u)) w.y = 0.f;
+                                    if (!(((seen & ~mute) >> (4 * k + 2 * h)) & 1u)) y.x = w.x * V_LEAST;
+                                    if (!(((seen & ~mute) >> (4 * k + 2 * h + 1)) & 1u)) y.y = w.y * V_LEAST;
+                                }
+                                most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));
+                                if constexpr (decltype(masked)::value) {
+                                    if (!(((seen & ~mute) >> (4 * k + 2 * h)) & 1u)) y.x = 0.f;
+                                    if (!(((seen & ~mute) >> (4 * k + 2 * h + 1)) & 1u)) y.y = 0.f;
+                                }
+                                add = __fadd2_rn(add, w);
+                                pk[2 * k + h] = half2_of(y.x, y.y);
+                            }
+                        }
+                    };
+                    if (masks) weigh(std::true_type{});
+                    else weigh(std::false_type{});
+                    if (__any_sync(0xffffffffu, most > 64.f)) {  // M moves for some row of the warp
+                        float top = M;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const float b = (mute >> k) & 1u ? V_LEAST : fabsf(table[PR_KEYS + 32 * ch + k]);
+                            const float x = fmaf(__uint_as_float(sr[k]) * table[32 * ch + k], c, __log2f(b));
+                            if ((seen >> k) & 1u) top = fmaxf(top, x);
+                        }
+                        const float f = most > 64.f ? ex2_approx(M - top) : 1.f;
+                        if (most > 64.f) M = top;
+                        l2 = make_float2(l2.x * f, l2.y * f);
+                        ptx::tmem_wait_st();
+                        for (int b = 0; b < ch; ++b) {  // this tile's weights so far
+                            uint32_t v[16];
+                            tmem_ld_x16(s_col + 16 * b, v);
+                            ptx::tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                const float2 w = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
+                                v[k] = half2_of(w.x * f, w.y * f);
+                            }
+                            tmem_st_x16(s_col + 16 * b, v);
+                        }
+                        if (j > s.j0)
+                            for (int b = 0; b < D / 16; ++b) {
+                                uint32_t v[16];
+                                tmem_ld_x16(o_col + 16 * b, v);
+                                ptx::tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                                tmem_st_x16(o_col + 16 * b, v);
+                            }
+                        if (masks) weigh(std::true_type{});
+                        else weigh(std::false_type{});
+                    }
+                    l2 = __fadd2_rn(l2, add);
+                    tmem_st_x16(s_col + 16 * ch, pk);
+                }
+                ptx::tmem_wait_st();
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(bar(P_FULL + t));
+            }
+            if (!ok) break;
+            // Q's products are done (the last S is here): the next segment's Q can go in
+            const PromptSegment cur = s;
+            const int64_t item_first = sched.split ? sched.at - cur.j1 : 0;  // (split: `at` is the end of this segment)
+            more = sched.next(s);
+            if (more) write_q(s);
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(O_FULL + t), seg_n & 1, s_abort));
+            ++seg_n;
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const float l = l2.x + l2.y;
+            T *o = static_cast<T *>(p.o) + tok * p.o_st + static_cast<int64_t>((cur.kvh << log_g) + (r & ((1 << log_g) - 1))) * p.o_sh;
+            auto store32 = [&](int b, const float (&v)[32]) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t u[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) u[h] = out2<T>(v[8 * k + 2 * h], v[8 * k + 2 * h + 1]);
+                    reinterpret_cast<uint4 *>(o + 32 * b)[k] = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            };
+            const bool whole = cur.j0 == 0 && cur.j1 == cur.tiles;
+            if (whole) {
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll 1
+                for (int b = 0; b < D / 32; ++b) {
+                    uint32_t u[32];
+                    ptx::tmem_ld_32x32b_x32(o_col + 32 * b, u);
+                    ptx::tmem_wait_ld();
+                    float v[32];
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = l != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
+                    if (live) store32(b, v);
+                }
+            } else {
+                const int piece = 2 * blockIdx.x + (cur.j0 == 0 ? 1 : 0);
+                float4 *acc = reinterpret_cast<float4 *>(work.acc) + (static_cast<int64_t>(piece) * 2 + t) * (D / 4) * 128 + row;
+#pragma unroll 1
+                for (int b = 0; b < D / 32; ++b) {
+                    uint32_t u[32];
+                    ptx::tmem_ld_32x32b_x32(o_col + 32 * b, u);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        acc[(8 * b + k) * 128] = make_float4(__uint_as_float(u[4 * k]), __uint_as_float(u[4 * k + 1]),
+                                                             __uint_as_float(u[4 * k + 2]), __uint_as_float(u[4 * k + 3]));
+                }
+                float *ml = work.ml + (static_cast<int64_t>(piece) * PR_ROWS + r) * 2;
+                ml[0] = M;
+                ml[1] = l;
+                const int first = sched.cta_of(item_first), pieces = sched.cta_of(item_first + cur.tiles - 1) - first + 1;
+                __threadfence();
+                if (!(ok = group_sync(JOIN, joins++))) break;
+                if (threadIdx.x == 0) {
+                    const int old = atomicAdd(work.counters + first, 1);
+                    s_last = old == pieces - 1;
+                    if (old == pieces - 1) work.counters[first] = 0;  // ready for the next launch
+                }
+                if (!(ok = group_sync(JOIN, joins++))) break;
+                const bool last = *static_cast<volatile int *>(&s_last) != 0;  // written again after the next joint's first barrier
+                if (last) {
+                    __threadfence();
+                    auto piece_of = [&](int k) { return static_cast<int64_t>(2 * (first + k) + (k == 0 ? 1 : 0)); };
+                    float top = M_NONE;
+                    for (int k = 0; k < pieces; ++k) top = fmaxf(top, __ldcg(work.ml + (piece_of(k) * PR_ROWS + r) * 2));
+                    float sum = 0.f;
+                    for (int k = 0; k < pieces; ++k) {
+                        const float *x = work.ml + (piece_of(k) * PR_ROWS + r) * 2;
+                        sum += __ldcg(x + 1) * ex2_approx(__ldcg(x) - top);
+                    }
+                    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll 1
+                    for (int b = 0; b < D / 32; ++b) {
+                        float v[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+                        for (int k = 0; k < pieces; ++k) {
+                            const float f = ex2_approx(__ldcg(work.ml + (piece_of(k) * PR_ROWS + r) * 2) - top);
+                            const float4 *src = reinterpret_cast<const float4 *>(work.acc) + (piece_of(k) * 2 + t) * (D / 4) * 128 + row;
+#pragma unroll
+                            for (int h = 0; h < 8; ++h) {
+                                const float4 a = __ldcg(src + (8 * b + h) * 128);
+                                v[4 * h] = fmaf(a.x, f, v[4 * h]);
+                                v[4 * h + 1] = fmaf(a.y, f, v[4 * h + 1]);
+                                v[4 * h + 2] = fmaf(a.z, f, v[4 * h + 2]);
+                                v[4 * h + 3] = fmaf(a.w, f, v[4 * h + 3]);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = sum != 0.f ? v[k] * inv : 0.f;
+                        if (live) store32(b, v);
+                    }
+                }
+            }
+            ptx::tc_fence_before();
+        }
+    } else if (warp < PR_MMA) {
+        // ==== converters: position tiles to fp16 in shared memory ====================================
+        const int w = warp - PR_CONVERT, me = w * 32 + lane;
+        constexpr int LOADS = 4 * KC;  // 16-byte loads of a K or V tile per thread: rows 32 x + 8 w + lane / 4
+        PromptSegment s;
+        int j = 0;
+        bool more = sched.next(s);
+        if (more) j = s.j0;
+        // Look-up of position `me` of the tile that the cursor (s, j) is at: pool row, block id
+        int blk = -1, slot = 0, kvh = 0;
+        auto lookup = [&] {
+            blk = -1;
+            if (!more) return;
+            const int pos = j * PR_KEYS + me;
+            // positions that some row of the item sees
+            const int64_t seen = min(static_cast<int64_t>(s.context), static_cast<int64_t>(s.offset) + min(s.q_len, (s.i + 1) * sched.tok));
+            kvh = s.kvh;
+            if (pos < seen) {
+                const int page = pos / p.block_size;
+                slot = pos - page * p.block_size;
+                blk = __ldcg(p.block_table + s.e * p.bt_stride + page);
+                if (blk < 0 || blk >= p.num_blocks) {
+                    report_status(LSE_ERR_INVALID_ARG);
+                    blk = -1;
+                }
+            }
+        };
+        auto advance = [&] {
+            if (!more) return;
+            if (++j == s.j1) {
+                more = sched.next(s);
+                if (more) j = s.j0;
+            }
+        };
+        float sk = 0.f, sv = 0.f;
+        bool dead = true;
+        int n = 0;
+        // publishes the looked-up rows of tile n and reads their scales
+        auto enter = [&](int at) -> bool {
+            const int64_t cell = static_cast<int64_t>(max(blk, 0)) * p.H_kv + kvh;
+            s_rows[at & 1][me] = blk < 0 ? 0u : static_cast<uint32_t>(cell * p.block_size + slot);
+            dead = blk < 0;
+            sk = dead ? 0.f : __ldcg(p.k_scale + cell);
+            sv = dead ? 0.f : __ldcg(p.v_scale + cell);
+            return group_sync(ROWS, at);
+        };
+        uint4 kr[LOADS], vr[LOADS];
+        auto load = [&](uint4 (&dst)[LOADS], const int8_t *pool, int at) {
+#pragma unroll
+            for (int x = 0; x < LOADS; ++x) {
+                const int r = 32 * (x / KC) + 8 * w + (lane >> 2);
+                const int8_t *src = pool + static_cast<int64_t>(s_rows[at & 1][r]) * D + 64 * (x % KC) + 16 * (lane & 3);
+                asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(dst[x].x), "=r"(dst[x].y), "=r"(dst[x].z), "=r"(dst[x].w) : "l"(src));
+            }
+        };
+        auto convert = [&](const uint4 (&src)[LOADS], uint8_t *tile) {
+#pragma unroll
+            for (int x = 0; x < LOADS; ++x) {
+                const int r = 32 * (x / KC) + 8 * w + (lane >> 2);
+                uint8_t *dst = tile + (x % KC) * (128 * 128) + r * 128;
+                const uint32_t u[4] = {src[x].x ^ 0x80808080u, src[x].y ^ 0x80808080u, src[x].z ^ 0x80808080u, src[x].w ^ 0x80808080u};
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<uint4 *>(dst + (((2 * (lane & 3) + h) ^ (r & 7)) << 4)) =
+                        make_uint4(codes_lo(u[2 * h]), codes_hi(u[2 * h]), codes_lo(u[2 * h + 1]), codes_hi(u[2 * h + 1]));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        bool running = more;
+        if (running) {
+            lookup();
+            running = enter(0);
+            load(kr, p.k_pool, 0);
+            load(vr, p.v_pool, 0);
+            advance();
+        }
+        while (running) {
+            const bool ahead = more;  // there is a tile n + 1
+            const float sk_now = sk, sv_now = sv;
+            const bool dead_now = dead;
+            lookup();
+            // ---- the scale table of tile n
+            float *table = table_of(n);
+            const bool mute = !dead_now && fabsf(sv_now) < V_LEAST;
+            table[me] = sk_now;
+            table[PR_KEYS + me] = dead_now || mute ? V_LEAST : sv_now;
+            const uint32_t dead_bits = __ballot_sync(0xffffffffu, dead_now), mute_bits = __ballot_sync(0xffffffffu, mute);
+            if (lane == 0) {
+                reinterpret_cast<uint32_t *>(table + 2 * PR_KEYS)[w] = dead_bits;
+                reinterpret_cast<uint32_t *>(table + 2 * PR_KEYS)[4 + w] = mute_bits;
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(TABLE_FULL + n % PR_TABLES));
+            bool ok = n < 2 || ptx::mbar_wait(bar(K_EMPTY + (n & 1)), ((n >> 1) - 1) & 1, s_abort);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            convert(kr, s_base + S::K + (n & 1) * S::TILE);
+            if (lane == 0) ptx::mbar_arrive(bar(K_FULL + (n & 1)));
+            if (ahead) {
+                if (!enter(n + 1)) break;
+                load(kr, p.k_pool, n + 1);
+            }
+            ok = n < 2 || ptx::mbar_wait(bar(V_EMPTY + (n & 1)), ((n >> 1) - 1) & 1, s_abort);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            convert(vr, s_base + S::V + (n & 1) * S::TILE);
+            if (lane == 0) ptx::mbar_arrive(bar(V_FULL + (n & 1)));
+            if (ahead) load(vr, p.v_pool, n + 1);
+            advance();
+            ++n;
+            running = ahead;
+        }
+    } else if (lane == 0) {
+        // ==== the MMA issuer ==========================================================================
+        int n = 0, seg_n = 0;
+        PromptSegment s;
+        bool ok = true;
+        auto qk = [&](int t, int at) {  // S_t = Q_t K(at)^T
+            const uint32_t q = base + S::Q + t * S::TILE, k = base + S::K + (at & 1) * S::TILE;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                const uint32_t off = (x >> 2) * (128 * 128) + (x & 3) * 32;
+                mma_f16_ss(tmem + 128 * t, ptx::smem_desc_sw128(q + off), ptx::smem_desc_sw128(k + off), ID_S, x > 0);
+            }
+            ptx::mma_commit(bar(S_FULL + t));
+            if (t == 1) ptx::mma_commit(bar(K_EMPTY + (at & 1)));
+        };
+        while (ok && sched.next(s)) {
+            const int tiles = s.j1 - s.j0;
+            for (int t = 0; t < 2 && ok; ++t) {
+                ok = ptx::mbar_wait(bar(Q_FULL + t), seg_n & 1, s_abort) && ptx::mbar_wait(bar(K_FULL + (n & 1)), (n >> 1) & 1, s_abort);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                qk(t, n);
+            }
+            for (int j = 0; j < tiles && ok; ++j, ++n) {
+                for (int t = 0; t < 2 && ok; ++t) {
+                    ok = ptx::mbar_wait(bar(V_FULL + (n & 1)), (n >> 1) & 1, s_abort) && ptx::mbar_wait(bar(P_FULL + t), n & 1, s_abort);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    const uint32_t v = base + S::V + (n & 1) * S::TILE;
+#pragma unroll
+                    for (int x = 0; x < PR_KEYS / 16; ++x)
+                        ptx::mma_bf16_ts(tmem + O_COL + 128 * t, tmem + 128 * t + 8 * x, desc_mn_sw128(v + 2048 * x, 128 * 128), ID_O, j > 0 || x > 0);
+                    if (t == 1) ptx::mma_commit(bar(V_EMPTY + (n & 1)));
+                    if (j + 1 < tiles) {
+                        ok = ptx::mbar_wait(bar(K_FULL + ((n + 1) & 1)), ((n + 1) >> 1) & 1, s_abort);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+                        qk(t, n + 1);
+                    } else {
+                        ptx::mma_commit(bar(O_FULL + t));
+                    }
+                }
+            }
+            ++seg_n;
+        }
+        ptx::mma_commit(bar(DRAIN));
+        ptx::mbar_drain(bar(DRAIN), 0);
+    }
+    ptx::tc_fence_before();
+    ptx::cta_sync_roles(bar(DONE));
+    if (warp == PR_MMA) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace kv8
+}  // namespace lse

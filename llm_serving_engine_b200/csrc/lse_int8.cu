@@ -932,6 +932,7 @@ int lse_set_wait_limit(int device, long long cycles) {
     }
     const long long v = cycles > 0 ? cycles : kWaitLimitCycles;
     e = cudaMemcpyToSymbol(g_wait_limit, &v, sizeof(v));
+    if (e == cudaSuccess) e = kv8_set_wait_limit(v);
     if (prev != device) cudaSetDevice(prev);
     if (e != cudaSuccess) { set_cuda_error(e, "lse_set_wait_limit"); return LSE_ERR_CUDA; }
     return LSE_OK;

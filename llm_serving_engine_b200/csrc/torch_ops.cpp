@@ -328,7 +328,8 @@ at::Tensor kv8_paged_attention(const at::Tensor &q, const at::Tensor &k, const a
     check_table(block_table, dev, what);
     const int dt = dtype_code(q);
     const int64_t E = block_table.size(0);
-    TORCH_CHECK(q.dim() == 3 && q.size(2) == c.D(), what, ": q must be [H, tokens, D] with the cache's D");
+    TORCH_CHECK(q.dim() == 3 && q.size(0) % c.H_kv() == 0 && q.size(2) == c.D(), what,
+                ": q must be [H, tokens, D] with the cache's D");
     check_i32(context_len, E, dev, what, "context_len");
     check_i32(query_offset, E, dev, what, "query_offset");
     check_i32(q_start, E, dev, what, "q_start");
@@ -338,13 +339,16 @@ at::Tensor kv8_paged_attention(const at::Tensor &q, const at::Tensor &k, const a
     at::Tensor o = at::empty({q.size(0), q.size(1), c.D()}, q.options());
     if (E == 0 || q.size(0) == 0 || q.size(1) == 0) return o;
     const at::Tensor x = rows16(q);
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const size_t ws_bytes = lse_kv8_paged_attention_workspace(q.size(0), c.H_kv(), c.D());
+    const at::Tensor ws = counters_workspace(1, ws_bytes, q, st);
     check_launch(lse_kv8_paged_attention(x.data_ptr(), dt, q.size(1), q.size(0), c.D(), x.stride(0), x.stride(1),
                                          k.data_ptr<int8_t>(), v.data_ptr<int8_t>(), k_scale.data_ptr<float>(),
                                          v_scale.data_ptr<float>(), c.num_blocks(), c.block_size(), c.H_kv(),
                                          block_table.data_ptr<int>(), block_table.stride(0), block_table.size(1),
                                          context_len.data_ptr<int>(), query_offset.data_ptr<int>(), q_start.data_ptr<int>(),
                                          q_len.data_ptr<int>(), E, static_cast<float>(scale), o.data_ptr(), o.stride(0),
-                                         o.stride(1), nullptr, 0, at::cuda::getCurrentCUDAStream(dev.index()).stream()),
+                                         o.stride(1), ws.data_ptr(), ws_bytes, st),
                  "lse_kv8_paged_attention");
     return o;
 }
