@@ -140,14 +140,15 @@ int launch_prompt(const kv8::AttnParams &p, void *workspace, int sms, cudaStream
     w.acc = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + prompt_counter_bytes(sms));
     w.ml = w.acc + 2ll * sms * kv8::PR_ROWS * D;
     constexpr int smem = kv8::PromptSmem<D>::BYTES;
-    cudaError_t e = cudaFuncSetAttribute(kv8::prompt_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const auto kernel = p.block_size % 16 == 0 ? kv8::prompt_kernel<D, T, true> : kv8::prompt_kernel<D, T, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return finish(e, "kv8_paged_attention attributes");
     int log_g = 0;
     while ((1 << log_g) < p.H / p.H_kv) ++log_g;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     host::launch_config(cfg, attr, dim3(static_cast<unsigned>(sms)), dim3(kv8::PR_THREADS), smem, st);
-    return finish(cudaLaunchKernelEx(&cfg, kv8::prompt_kernel<D, T>, p, w, log_g), "kv8_paged_attention launch");
+    return finish(cudaLaunchKernelEx(&cfg, kernel, p, w, log_g), "kv8_paged_attention launch");
 }
 
 }  // namespace

@@ -58,11 +58,12 @@ struct PromptSmem {
 struct PromptSegment {
     int e, kvh, i, j0, j1, tiles;
     int q_start, q_len, offset, context;
+    int64_t item;  // split: the item's first tile
 };
 
-// The schedule, the same in every role; see the header comment.
+// The schedule, the same in every role; see the header comment.  Each warp keeps a copy in shared
+// memory (its fields would be registers that the softmax has no room for).
 struct PromptSchedule {
-    const AttnParams *p;
     int tok;            // tokens per item
     int64_t at, end, total, active;  // split: this CTA's run of tiles; whole: its next item and their number
     bool split;
@@ -78,44 +79,45 @@ struct PromptSchedule {
         const int64_t seen = min(static_cast<int64_t>(context), static_cast<int64_t>(offset) + min(q_len, (i + 1) * tok));
         return static_cast<int>(max(static_cast<int64_t>(1), (seen + PR_KEYS - 1) / PR_KEYS));
     }
-    __device__ __forceinline__ void load_entry() {
-        if (e >= p->E) return;
-        q_start = __ldcg(p->q_start + e);
-        q_len = max(__ldcg(p->q_len + e), 0);
-        offset = __ldcg(p->query_offset + e);
-        context = context_of(*p, e);
+    __device__ __forceinline__ void load_entry(const AttnParams &p) {
+        if (e >= p.E) return;
+        q_start = __ldcg(p.q_start + e);
+        q_len = max(__ldcg(p.q_len + e), 0);
+        offset = __ldcg(p.query_offset + e);
+        context = context_of(p, e);
         nq = (q_len + tok - 1) / tok;
     }
-    __device__ __forceinline__ bool next(PromptSegment &s) {
+    __device__ __forceinline__ bool next(const AttnParams &p, PromptSegment &s) {
         if (at >= end) return false;
         if (split) {
             const int n = tiles_of(context, offset, q_len, tok, i);
             s.j0 = static_cast<int>(at - first);
             s.j1 = static_cast<int>(min(end, first + n) - first);
             fill(s, n);
+            s.item = first;
             at = first + s.j1;
             if (s.j1 == n) {  // the next item
                 first += n;
                 if (++i == nq) {
                     i = 0;
-                    if (++kvh == p->H_kv) {
+                    if (++kvh == p.H_kv) {
                         kvh = 0;
                         do {
                             ++e;
-                            load_entry();
-                        } while (e < p->E && nq == 0);
+                            load_entry(p);
+                        } while (e < p.E && nq == 0);
                     }
                 }
             }
         } else {
-            while (at >= first + static_cast<int64_t>(nq) * p->H_kv) {
-                first += static_cast<int64_t>(nq) * p->H_kv;
+            while (at >= first + static_cast<int64_t>(nq) * p.H_kv) {
+                first += static_cast<int64_t>(nq) * p.H_kv;
                 ++e;
-                load_entry();
+                load_entry(p);
             }
             const int k = static_cast<int>(at - first);
-            kvh = k % p->H_kv;
-            i = nq - 1 - k / p->H_kv;  // the longest first
+            kvh = k % p.H_kv;
+            i = nq - 1 - k / p.H_kv;  // the longest first
             s.j0 = 0;
             s.j1 = tiles_of(context, offset, q_len, tok, i);
             fill(s, s.j1);
@@ -177,8 +179,9 @@ __device__ __forceinline__ uint32_t out2(float lo, float hi) {  // two elements 
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptWork work, const int log_g) {
+// PAGED16: block_size is a multiple of 16, so that 16 positions share a page and its scales.
+template <int D, typename T, bool PAGED16>
+__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ PromptWork work, const int log_g) {
     using S = PromptSmem<D>;
     constexpr float M_NONE = -1e30f, V_LEAST = 5.0487098e-29f;  // as in the decode kernel
     constexpr int KC = D / 64;                    // 64-dim halves of a row
@@ -196,6 +199,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
     __shared__ int s_abort_word, s_last;
     __shared__ int64_t s_sum[PR_WARPS][2];
     __shared__ int64_t s_found[3];
+    __shared__ PromptSchedule s_sched[PR_WARPS];
+    __shared__ PromptSegment s_seg[PR_WARPS][2];
     const uint32_t base = (ptx::smem_u32(s_raw) + 1023u) & ~1023u;
     uint8_t *const s_base = s_raw + (base - ptx::smem_u32(s_raw));
     volatile int *s_abort = &s_abort_word;
@@ -228,19 +233,24 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the cache and the lengths come from earlier kernels
 
+    // One lane waits for its warp (32 that poll would part and come back one by one).
+    auto warp_wait = [&](int b, int phase) {
+        int ok = 0;
+        if (lane == 0) ok = ptx::mbar_wait(bar(b), phase & 1, s_abort);
+        return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    };
     // A barrier of some warps that, unlike bar.sync, gives up with the CTA: every warp arrives once a phase.
     auto group_sync = [&](int b, int phase) {
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(b));
-        const bool ok = ptx::mbar_wait(bar(b), phase & 1, s_abort);
-        return static_cast<bool>(__all_sync(0xffffffffu, ok));
+        return warp_wait(b, phase);
     };
 
     // ---- the schedule ------------------------------------------------------------------------------
-    PromptSchedule sched;
-    sched.p = &p;
-    sched.tok = PR_ROWS >> log_g;
+    const int item_tokens = PR_ROWS >> log_g;
     {
+        PromptSchedule sched;
+        sched.tok = item_tokens;
         auto entry = [&](int e, int64_t &tiles, int64_t &items) {
             tiles = items = 0;
             if (e >= p.E) return;
@@ -318,7 +328,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             }
             if (sched.at < sched.end) {
                 sched.e = static_cast<int>(s_found[0]);
-                sched.load_entry();
+                sched.load_entry(p);
                 const int64_t off = sched.at - s_found[1];
                 sched.kvh = static_cast<int>(off / s_found[2]);
                 sched.first = s_found[1] + sched.kvh * s_found[2];
@@ -330,7 +340,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             sched.at = blockIdx.x;
             sched.end = items_all;
         }
+        if (lane == 0) s_sched[warp] = sched;
     }
+    // The k-th segment of this CTA into this warp's slot k & 1; false when there is none.
+    auto next_segment = [&](int k) {
+        __syncwarp();
+        int more = 0;
+        if (lane == 0) more = s_sched[warp].next(p, s_seg[warp][k & 1]);
+        return __shfl_sync(0xffffffffu, more, 0) != 0;
+    };
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
@@ -344,11 +362,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + O_COL + 128 * t;
         uint8_t *const q_tile = s_base + S::Q + t * S::TILE;
         int n = 0, seg_n = 0, joins = 0;  // position tiles, segments and joint barriers so far
-        PromptSegment s;
         float back = 1.f;
         // Writes this row of Q as fp16 (scaled to [1, 2) at its largest by a power of two for bf16).
         auto write_q = [&](const PromptSegment &x) {
-            const int r = 128 * t + row, in = x.i * sched.tok + (r >> log_g), tok = x.q_start + in;
+            const int r = 128 * t + row, in = x.i * item_tokens + (r >> log_g), tok = x.q_start + in;
             const bool live = in < x.q_len && tok >= 0 && tok < p.tokens;
             const T *src = static_cast<const T *>(p.q) + tok * p.q_st + static_cast<int64_t>((x.kvh << log_g) + (r & ((1 << log_g) - 1))) * p.q_sh;
             float down = 1.f;
@@ -391,20 +408,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             if (lane == 0) ptx::mbar_arrive(bar(Q_FULL + t));
         };
         bool ok = true;
-        bool more = sched.next(s);
-        if (more) write_q(s);
+        bool more = next_segment(0);
+        if (more) write_q(s_seg[warp][0]);
         while (more && ok) {
-            const int r = 128 * t + row, in = s.i * sched.tok + (r >> log_g);
+            const PromptSegment &s = s_seg[warp][seg_n & 1];
+            const int r = 128 * t + row, in = s.i * item_tokens + (r >> log_g);
             const int tok = s.q_start + in;
             const bool live = in < s.q_len && tok >= 0 && tok < p.tokens;
             const int limit = live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(s.context), static_cast<int64_t>(s.offset) + in + 1))) : 0;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const float c = p.scale_log2 * back;
             float M = M_NONE;
-            float2 l2 = make_float2(0.f, 0.f);
-            for (int j = s.j0; j < s.j1; ++j, ++n) {
-                ok = ptx::mbar_wait(bar(TABLE_FULL + n % PR_TABLES), (n / PR_TABLES) & 1, s_abort) && ptx::mbar_wait(bar(S_FULL + t), n & 1, s_abort);
-                ok = __all_sync(0xffffffffu, ok);
+            float l[2] = {0.f, 0.f};
+            const int j0 = s.j0, j1 = s.j1;
+            for (int j = j0; j < j1; ++j, ++n) {
+                ok = warp_wait(TABLE_FULL + n % PR_TABLES, n / PR_TABLES) && warp_wait(S_FULL + t, n);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 if (!warp_live) {  // no row of this warp is stored: its weights do not matter
@@ -415,87 +433,88 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 const uint32_t *bits = reinterpret_cast<const uint32_t *>(table + 2 * PR_KEYS);  // 4 words dead, 4 words mute
                 const int pos = j * PR_KEYS;
 #pragma unroll 1
-                for (int ch = 0; ch < 4; ++ch) {
+                for (int ch = 0; ch < 4; ++ch) {  // 32 positions: S to registers, the weights back as fp16
                     uint32_t sr[32];
                     ptx::tmem_ld_32x32b_x32(s_col + 32 * ch, sr);
                     const uint32_t dead = bits[ch], mute = bits[4 + ch];
                     const int left = limit - pos - 32 * ch;
                     const uint32_t seen = (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u) & ~dead;
                     const bool masks = __any_sync(0xffffffffu, (seen & ~mute) != ~0u);
-                    const float4 *sk = reinterpret_cast<const float4 *>(table + 32 * ch), *sv = reinterpret_cast<const float4 *>(table + PR_KEYS + 32 * ch);
-                    ptx::tmem_wait_ld();
+                    const float *sk = table + 32 * ch, *sv = table + PR_KEYS + 32 * ch;
                     uint32_t pk[16];
-                    float most;
-                    float2 add;
-                    auto weigh = [&](auto masked) {
-                        most = 0.f;
-                        add = make_float2(0.f, 0.f);
-                        const float2 c2 = make_float2(c, c), m2 = make_float2(-M, -M);
+                    float add[2];
+                    ptx::tmem_wait_ld();
+                    while (true) {
+                        bool over;  // a weight is over 2^6 as it would meet V
+                        add[0] = add[1] = 0.f;
+                        if (!masks) {
+                            __half2 most = __float2half2_rn(0.f);
+                            float f = 0.f, v = 0.f;
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float4 a = sk[k], b = sv[k];
+                            for (int k = 0; k < 16; ++k) {
+                                float w[2], y[2];
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float2 x = make_float2(__uint_as_float(sr[4 * k + 2 * h]), __uint_as_float(sr[4 * k + 2 * h + 1]));
-                                float2 w = __ffma2_rn(__fmul2_rn(x, h ? make_float2(a.z, a.w) : make_float2(a.x, a.y)), c2, m2);
-                                w.x = ex2_approx(w.x);
-                                w.y = ex2_approx(w.y);
-                                const float2 v = h ? make_float2(b.z, b.w) : make_float2(b.x, b.y);
-                                float2 y = __fmul2_rn(w, v);
-                                if constexpr (decltype(masked)::value) {
-                                    if (!((seen >> (4 * k + 2 * h)) & 1u)) w.x = 0.f;
-                                    if (!((seen >> (4 * k + 2 * h + 1)) & 1u)) w.y = 0.f;
-                                    if (!(((seen & ~mute) >> (4 * k + 2 * h)) & 1u)) y.x = w.x * V_LEAST;
-                                    if (!(((seen & ~mute) >> (4 * k + 2 * h + 1)) & 1u)) y.y = w.y * V_LEAST;
+                                for (int h = 0; h < 2; ++h) {
+                                    if (!PAGED16 || (2 * k + h) % 16 == 0) {  // PAGED16: 16 positions share a page
+                                        f = sk[2 * k + h] * c;
+                                        v = sv[2 * k + h];
+                                    }
+                                    w[h] = ex2_approx(fmaf(__uint_as_float(sr[2 * k + h]), f, -M));
+                                    add[h] += w[h];
+                                    y[h] = w[h] * v;
                                 }
-                                most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));
-                                if constexpr (decltype(masked)::value) {
-                                    if (!(((seen & ~mute) >> (4 * k + 2 * h)) & 1u)) y.x = 0.f;
-                                    if (!(((seen & ~mute) >> (4 * k + 2 * h + 1)) & 1u)) y.y = 0.f;
+                                pk[k] = half2_of(y[0], y[1]);
+                                most = __hmax2(most, *reinterpret_cast<const __half2 *>(&pk[k]));
+                            }
+                            over = __hgt(__hmax(__low2half(most), __high2half(most)), __float2half_rn(64.f));
+                        } else {  // unseen: no weight; mute pages: values of 0
+                            over = false;
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                float y[2];
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const bool on = (seen >> (2 * k + h)) & 1u;
+                                    const float w = on ? ex2_approx(fmaf(__uint_as_float(sr[2 * k + h]), sk[2 * k + h] * c, -M)) : 0.f;
+                                    add[h] += w;
+                                    y[h] = on ? w * sv[2 * k + h] : 0.f;
+                                    over |= y[h] > 64.f;
+                                    if ((mute >> (2 * k + h)) & 1u) y[h] = 0.f;
                                 }
-                                add = __fadd2_rn(add, w);
-                                pk[2 * k + h] = half2_of(y.x, y.y);
+                                pk[k] = half2_of(y[0], y[1]);
                             }
                         }
-                    };
-                    if (masks) weigh(std::true_type{});
-                    else weigh(std::false_type{});
-                    if (__any_sync(0xffffffffu, most > 64.f)) {  // M moves for some row of the warp
+                        if (!__any_sync(0xffffffffu, over)) break;
+                        // M moves for some row of the warp
                         float top = M;
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
-                            const float b = (mute >> k) & 1u ? V_LEAST : fabsf(table[PR_KEYS + 32 * ch + k]);
-                            const float x = fmaf(__uint_as_float(sr[k]) * table[32 * ch + k], c, __log2f(b));
+                            const float x = fmaf(__uint_as_float(sr[k]) * sk[k], c, __log2f(fabsf(sv[k])));
                             if ((seen >> k) & 1u) top = fmaxf(top, x);
                         }
-                        const float f = most > 64.f ? ex2_approx(M - top) : 1.f;
-                        if (most > 64.f) M = top;
-                        l2 = make_float2(l2.x * f, l2.y * f);
+                        const float f = over ? ex2_approx(M - top) : 1.f;
+                        if (over) M = top;
+                        l[0] *= f;
+                        l[1] *= f;
                         ptx::tmem_wait_st();
-                        for (int b = 0; b < ch; ++b) {  // this tile's weights so far
+                        // this tile's weights so far, and (past the first tile) the sums
+#pragma unroll 1
+                        for (int b = j > j0 ? 0 : D / 16; b < D / 16 + ch; ++b) {
                             uint32_t v[16];
-                            tmem_ld_x16(s_col + 16 * b, v);
+                            const bool sums = b < D / 16;
+                            const uint32_t col = sums ? o_col + 16 * b : s_col + 16 * (b - D / 16);
+                            tmem_ld_x16(col, v);
                             ptx::tmem_wait_ld();
 #pragma unroll
                             for (int k = 0; k < 16; ++k) {
                                 const float2 w = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
-                                v[k] = half2_of(w.x * f, w.y * f);
+                                v[k] = sums ? __float_as_uint(__uint_as_float(v[k]) * f) : half2_of(w.x * f, w.y * f);
                             }
-                            tmem_st_x16(s_col + 16 * b, v);
+                            tmem_st_x16(col, v);
                         }
-                        if (j > s.j0)
-                            for (int b = 0; b < D / 16; ++b) {
-                                uint32_t v[16];
-                                tmem_ld_x16(o_col + 16 * b, v);
-                                ptx::tmem_wait_ld();
-#pragma unroll
-                                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-                                tmem_st_x16(o_col + 16 * b, v);
-                            }
-                        if (masks) weigh(std::true_type{});
-                        else weigh(std::false_type{});
                     }
-                    l2 = __fadd2_rn(l2, add);
+                    l[0] += add[0];
+                    l[1] += add[1];
                     tmem_st_x16(s_col + 16 * ch, pk);
                 }
                 ptx::tmem_wait_st();
@@ -505,15 +524,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             }
             if (!ok) break;
             // Q's products are done (the last S is here): the next segment's Q can go in
-            const PromptSegment cur = s;
-            const int64_t item_first = sched.split ? sched.at - cur.j1 : 0;  // (split: `at` is the end of this segment)
-            more = sched.next(s);
-            if (more) write_q(s);
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(O_FULL + t), seg_n & 1, s_abort));
+            const PromptSegment &cur = s;
+            more = next_segment(seg_n + 1);
+            if (more) write_q(s_seg[warp][(seg_n + 1) & 1]);
+            ok = warp_wait(O_FULL + t, seg_n);
             ++seg_n;
             if (!ok) break;
             ptx::tc_fence_after();
-            const float l = l2.x + l2.y;
+            const float sum_w = l[0] + l[1];
             T *o = static_cast<T *>(p.o) + tok * p.o_st + static_cast<int64_t>((cur.kvh << log_g) + (r & ((1 << log_g) - 1))) * p.o_sh;
             auto store32 = [&](int b, const float (&v)[32]) {
 #pragma unroll
@@ -526,7 +544,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             };
             const bool whole = cur.j0 == 0 && cur.j1 == cur.tiles;
             if (whole) {
-                const float inv = l != 0.f ? 1.f / l : 0.f;
+                const float inv = sum_w != 0.f ? 1.f / sum_w : 0.f;
 #pragma unroll 1
                 for (int b = 0; b < D / 32; ++b) {
                     uint32_t u[32];
@@ -534,7 +552,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                     ptx::tmem_wait_ld();
                     float v[32];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = l != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
+                    for (int k = 0; k < 32; ++k) v[k] = sum_w != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
                     if (live) store32(b, v);
                 }
             } else {
@@ -552,8 +570,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 }
                 float *ml = work.ml + (static_cast<int64_t>(piece) * PR_ROWS + r) * 2;
                 ml[0] = M;
-                ml[1] = l;
-                const int first = sched.cta_of(item_first), pieces = sched.cta_of(item_first + cur.tiles - 1) - first + 1;
+                ml[1] = sum_w;
+                const int first = s_sched[warp].cta_of(cur.item), pieces = s_sched[warp].cta_of(cur.item + cur.tiles - 1) - first + 1;
                 __threadfence();
                 if (!(ok = group_sync(JOIN, joins++))) break;
                 if (threadIdx.x == 0) {
@@ -603,18 +621,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         // ==== converters: position tiles to fp16 in shared memory ====================================
         const int w = warp - PR_CONVERT, me = w * 32 + lane;
         constexpr int LOADS = 4 * KC;  // 16-byte loads of a K or V tile per thread: rows 32 x + 8 w + lane / 4
-        PromptSegment s;
-        int j = 0;
-        bool more = sched.next(s);
-        if (more) j = s.j0;
+        int j = 0, seg_n = 0;
+        bool more = next_segment(0);
+        if (more) j = s_seg[warp][0].j0;
         // Look-up of position `me` of the tile that the cursor (s, j) is at: pool row, block id
         int blk = -1, slot = 0, kvh = 0;
         auto lookup = [&] {
             blk = -1;
             if (!more) return;
+            const PromptSegment &s = s_seg[warp][seg_n & 1];
             const int pos = j * PR_KEYS + me;
             // positions that some row of the item sees
-            const int64_t seen = min(static_cast<int64_t>(s.context), static_cast<int64_t>(s.offset) + min(s.q_len, (s.i + 1) * sched.tok));
+            const int64_t seen = min(static_cast<int64_t>(s.context), static_cast<int64_t>(s.offset) + min(s.q_len, (s.i + 1) * item_tokens));
             kvh = s.kvh;
             if (pos < seen) {
                 const int page = pos / p.block_size;
@@ -628,9 +646,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         };
         auto advance = [&] {
             if (!more) return;
-            if (++j == s.j1) {
-                more = sched.next(s);
-                if (more) j = s.j0;
+            if (++j == s_seg[warp][seg_n & 1].j1) {
+                more = next_segment(++seg_n);
+                if (more) j = s_seg[warp][seg_n & 1].j0;
             }
         };
         float sk = 0.f, sv = 0.f;
@@ -694,16 +712,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar(TABLE_FULL + n % PR_TABLES));
-            bool ok = n < 2 || ptx::mbar_wait(bar(K_EMPTY + (n & 1)), ((n >> 1) - 1) & 1, s_abort);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (n >= 2 && !warp_wait(K_EMPTY + (n & 1), (n >> 1) - 1)) break;
             convert(kr, s_base + S::K + (n & 1) * S::TILE);
             if (lane == 0) ptx::mbar_arrive(bar(K_FULL + (n & 1)));
             if (ahead) {
                 if (!enter(n + 1)) break;
                 load(kr, p.k_pool, n + 1);
             }
-            ok = n < 2 || ptx::mbar_wait(bar(V_EMPTY + (n & 1)), ((n >> 1) - 1) & 1, s_abort);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (n >= 2 && !warp_wait(V_EMPTY + (n & 1), (n >> 1) - 1)) break;
             convert(vr, s_base + S::V + (n & 1) * S::TILE);
             if (lane == 0) ptx::mbar_arrive(bar(V_FULL + (n & 1)));
             if (ahead) load(vr, p.v_pool, n + 1);
@@ -726,7 +742,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             ptx::mma_commit(bar(S_FULL + t));
             if (t == 1) ptx::mma_commit(bar(K_EMPTY + (at & 1)));
         };
-        while (ok && sched.next(s)) {
+        while (ok && s_sched[warp].next(p, s)) {
             const int tiles = s.j1 - s.j0;
             for (int t = 0; t < 2 && ok; ++t) {
                 ok = ptx::mbar_wait(bar(Q_FULL + t), seg_n & 1, s_abort) && ptx::mbar_wait(bar(K_FULL + (n & 1)), (n >> 1) & 1, s_abort);
