@@ -233,17 +233,19 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the cache and the lengths come from earlier kernels
 
-    // One lane waits for its warp (32 that poll would part and come back one by one).
+    // One lane waits for its warp (32 that poll would part and come back one by one).  A wait that
+    // runs out raises the CTA's abort flag, and every later one returns at once: the roles run their
+    // loops to the end on whatever is in shared memory (all of it in bounds, the result undefined) and
+    // meet at the exit, with no branch on it that would make their control non-uniform.
     auto warp_wait = [&](int b, int phase) {
-        int ok = 0;
-        if (lane == 0) ok = ptx::mbar_wait(bar(b), phase & 1, s_abort);
-        return __shfl_sync(0xffffffffu, ok, 0) != 0;
+        if (lane == 0) ptx::mbar_wait(bar(b), phase & 1, s_abort);
+        __syncwarp();
     };
     // A barrier of some warps that, unlike bar.sync, gives up with the CTA: every warp arrives once a phase.
     auto group_sync = [&](int b, int phase) {
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(b));
-        return warp_wait(b, phase);
+        warp_wait(b, phase);
     };
 
     // ---- the schedule ------------------------------------------------------------------------------
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
         __syncwarp();
         int more = 0;
         if (lane == 0) more = s_sched[warp].next(p, s_seg[warp][k & 1]);
-        return __shfl_sync(0xffffffffu, more, 0) != 0;
+        return __reduce_max_sync(0xffffffffu, more) != 0;
     };
     ptx::tc_fence_before();
     __syncthreads();
@@ -407,10 +409,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar(Q_FULL + t));
         };
-        bool ok = true;
         bool more = next_segment(0);
         if (more) write_q(s_seg[warp][0]);
-        while (more && ok) {
+        while (more) {
             const PromptSegment &s = s_seg[warp][seg_n & 1];
             const int r = 128 * t + row, in = s.i * item_tokens + (r >> log_g);
             const int tok = s.q_start + in;
@@ -422,8 +423,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             float l[2] = {0.f, 0.f};
             const int j0 = s.j0, j1 = s.j1;
             for (int j = j0; j < j1; ++j, ++n) {
-                ok = warp_wait(TABLE_FULL + n % PR_TABLES, n / PR_TABLES) && warp_wait(S_FULL + t, n);
-                if (!ok) break;
+                warp_wait(TABLE_FULL + n % PR_TABLES, n / PR_TABLES);
+                warp_wait(S_FULL + t, n);
                 ptx::tc_fence_after();
                 if (!warp_live) {  // no row of this warp is stored: its weights do not matter
                     if (lane == 0) ptx::mbar_arrive(bar(P_FULL + t));
@@ -522,14 +523,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(bar(P_FULL + t));
             }
-            if (!ok) break;
             // Q's products are done (the last S is here): the next segment's Q can go in
             const PromptSegment &cur = s;
             more = next_segment(seg_n + 1);
             if (more) write_q(s_seg[warp][(seg_n + 1) & 1]);
-            ok = warp_wait(O_FULL + t, seg_n);
+            warp_wait(O_FULL + t, seg_n);
             ++seg_n;
-            if (!ok) break;
             ptx::tc_fence_after();
             const float sum_w = l[0] + l[1];
             T *o = static_cast<T *>(p.o) + tok * p.o_st + static_cast<int64_t>((cur.kvh << log_g) + (r & ((1 << log_g) - 1))) * p.o_sh;
@@ -573,13 +572,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
                 ml[1] = sum_w;
                 const int first = s_sched[warp].cta_of(cur.item), pieces = s_sched[warp].cta_of(cur.item + cur.tiles - 1) - first + 1;
                 __threadfence();
-                if (!(ok = group_sync(JOIN, joins++))) break;
+                group_sync(JOIN, joins++);
                 if (threadIdx.x == 0) {
                     const int old = atomicAdd(work.counters + first, 1);
                     s_last = old == pieces - 1;
                     if (old == pieces - 1) work.counters[first] = 0;  // ready for the next launch
                 }
-                if (!(ok = group_sync(JOIN, joins++))) break;
+                group_sync(JOIN, joins++);
                 const bool last = *static_cast<volatile int *>(&s_last) != 0;  // written again after the next joint's first barrier
                 if (last) {
                     __threadfence();
@@ -655,13 +654,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
         bool dead = true;
         int n = 0;
         // publishes the looked-up rows of tile n and reads their scales
-        auto enter = [&](int at) -> bool {
+        auto enter = [&](int at) {
             const int64_t cell = static_cast<int64_t>(max(blk, 0)) * p.H_kv + kvh;
             s_rows[at & 1][me] = blk < 0 ? 0u : static_cast<uint32_t>(cell * p.block_size + slot);
             dead = blk < 0;
             sk = dead ? 0.f : __ldcg(p.k_scale + cell);
             sv = dead ? 0.f : __ldcg(p.v_scale + cell);
-            return group_sync(ROWS, at);
+            group_sync(ROWS, at);
         };
         uint4 kr[LOADS], vr[LOADS];
         auto load = [&](uint4 (&dst)[LOADS], const int8_t *pool, int at) {
@@ -690,7 +689,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
         bool running = more;
         if (running) {
             lookup();
-            running = enter(0);
+            enter(0);
             load(kr, p.k_pool, 0);
             load(vr, p.v_pool, 0);
             advance();
@@ -712,14 +711,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar(TABLE_FULL + n % PR_TABLES));
-            if (n >= 2 && !warp_wait(K_EMPTY + (n & 1), (n >> 1) - 1)) break;
+            if (n >= 2) warp_wait(K_EMPTY + (n & 1), (n >> 1) - 1);
             convert(kr, s_base + S::K + (n & 1) * S::TILE);
             if (lane == 0) ptx::mbar_arrive(bar(K_FULL + (n & 1)));
             if (ahead) {
-                if (!enter(n + 1)) break;
+                enter(n + 1);
                 load(kr, p.k_pool, n + 1);
             }
-            if (n >= 2 && !warp_wait(V_EMPTY + (n & 1), (n >> 1) - 1)) break;
+            if (n >= 2) warp_wait(V_EMPTY + (n & 1), (n >> 1) - 1);
             convert(vr, s_base + S::V + (n & 1) * S::TILE);
             if (lane == 0) ptx::mbar_arrive(bar(V_FULL + (n & 1)));
             if (ahead) load(vr, p.v_pool, n + 1);
@@ -727,53 +726,63 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             ++n;
             running = ahead;
         }
-    } else if (lane == 0) {
+    } else {
         // ==== the MMA issuer ==========================================================================
+        // The whole warp runs this role and one elected lane issues: with warp-uniform control the
+        // descriptors stay in uniform registers (a branch on lane 0 around the role cost 130 cycles an
+        // MMA, whatever its size; elected, 101 from shared memory and 73 with P from tensor memory).
+        uint32_t elected;
+        asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+        const bool lead = elected != 0;
+        const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), smem = __reduce_max_sync(0xffffffffu, base);  // uniform registers
         int n = 0, seg_n = 0;
-        PromptSegment s;
-        bool ok = true;
         auto qk = [&](int t, int at) {  // S_t = Q_t K(at)^T
-            const uint32_t q = base + S::Q + t * S::TILE, k = base + S::K + (at & 1) * S::TILE;
+            const uint32_t q = smem + S::Q + t * S::TILE, k = smem + S::K + (at & 1) * S::TILE;
+            if (lead) {
 #pragma unroll
-            for (int x = 0; x < D / 16; ++x) {
-                const uint32_t off = (x >> 2) * (128 * 128) + (x & 3) * 32;
-                mma_f16_ss(tmem + 128 * t, ptx::smem_desc_sw128(q + off), ptx::smem_desc_sw128(k + off), ID_S, x > 0);
+                for (int x = 0; x < D / 16; ++x) {
+                    const uint32_t off = (x >> 2) * (128 * 128) + (x & 3) * 32;
+                    mma_f16_ss(tm + 128 * t, ptx::smem_desc_sw128(q + off), ptx::smem_desc_sw128(k + off), ID_S, x > 0);
+                }
+                ptx::mma_commit(bar(S_FULL + t));
+                if (t == 1) ptx::mma_commit(bar(K_EMPTY + (at & 1)));
             }
-            ptx::mma_commit(bar(S_FULL + t));
-            if (t == 1) ptx::mma_commit(bar(K_EMPTY + (at & 1)));
+            __syncwarp();
         };
-        while (ok && s_sched[warp].next(p, s)) {
-            const int tiles = s.j1 - s.j0;
-            for (int t = 0; t < 2 && ok; ++t) {
-                ok = ptx::mbar_wait(bar(Q_FULL + t), seg_n & 1, s_abort) && ptx::mbar_wait(bar(K_FULL + (n & 1)), (n >> 1) & 1, s_abort);
-                if (!ok) break;
+        while (next_segment(seg_n)) {
+            const int tiles = __reduce_max_sync(0xffffffffu, s_seg[warp][seg_n & 1].j1 - s_seg[warp][seg_n & 1].j0);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                warp_wait(Q_FULL + t, seg_n);
+                if (t == 0) warp_wait(K_FULL + (n & 1), n >> 1);
                 ptx::tc_fence_after();
                 qk(t, n);
             }
-            for (int j = 0; j < tiles && ok; ++j, ++n) {
-                for (int t = 0; t < 2 && ok; ++t) {
-                    ok = ptx::mbar_wait(bar(V_FULL + (n & 1)), (n >> 1) & 1, s_abort) && ptx::mbar_wait(bar(P_FULL + t), n & 1, s_abort);
-                    if (!ok) break;
-                    ptx::tc_fence_after();
-                    const uint32_t v = base + S::V + (n & 1) * S::TILE;
+            for (int j = 0; j < tiles; ++j, ++n) {
+                warp_wait(V_FULL + (n & 1), n >> 1);
+                if (j + 1 < tiles) warp_wait(K_FULL + ((n + 1) & 1), (n + 1) >> 1);
 #pragma unroll
-                    for (int x = 0; x < PR_KEYS / 16; ++x)
-                        ptx::mma_bf16_ts(tmem + O_COL + 128 * t, tmem + 128 * t + 8 * x, desc_mn_sw128(v + 2048 * x, 128 * 128), ID_O, j > 0 || x > 0);
-                    if (t == 1) ptx::mma_commit(bar(V_EMPTY + (n & 1)));
-                    if (j + 1 < tiles) {
-                        ok = ptx::mbar_wait(bar(K_FULL + ((n + 1) & 1)), ((n + 1) >> 1) & 1, s_abort);
-                        if (!ok) break;
-                        ptx::tc_fence_after();
-                        qk(t, n + 1);
-                    } else {
-                        ptx::mma_commit(bar(O_FULL + t));
+                for (int t = 0; t < 2; ++t) {
+                    warp_wait(P_FULL + t, n);
+                    ptx::tc_fence_after();
+                    const uint32_t v = smem + S::V + (n & 1) * S::TILE;
+                    if (lead) {
+#pragma unroll
+                        for (int x = 0; x < PR_KEYS / 16; ++x)
+                            ptx::mma_bf16_ts(tm + O_COL + 128 * t, tm + 128 * t + 8 * x, desc_mn_sw128(v + 2048 * x, 128 * 128), ID_O, j > 0 || x > 0);
+                        if (t == 1) ptx::mma_commit(bar(V_EMPTY + (n & 1)));
+                        if (j + 1 == tiles) ptx::mma_commit(bar(O_FULL + t));
                     }
+                    __syncwarp();
+                    if (j + 1 < tiles) qk(t, n + 1);
                 }
             }
             ++seg_n;
         }
-        ptx::mma_commit(bar(DRAIN));
-        ptx::mbar_drain(bar(DRAIN), 0);
+        if (lead) {
+            ptx::mma_commit(bar(DRAIN));
+            ptx::mbar_drain(bar(DRAIN), 0);
+        }
     }
     ptx::tc_fence_before();
     ptx::cta_sync_roles(bar(DONE));
