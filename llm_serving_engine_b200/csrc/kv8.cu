@@ -294,6 +294,10 @@ int lse_kv8_paged_attention(const void *q, int dtype, int64_t tokens, int64_t H,
     if (!q || !o || !context_len || !query_offset || !q_start || !q_len) return LSE_ERR_INVALID_ARG;
     if ((rc = check_table(block_table, bt_stride, bt_cols, E, block_size))) return rc;
     if (tokens > INT32_MAX / 2) return LSE_ERR_UNSUPPORTED;
+    {  // the kernel counts position tiles in 32 bits: items of 256 rows times the tiles of the longest context
+        const int64_t items = tokens * (H / H_kv) / kv8::PR_ROWS + E, tiles = bt_cols * block_size / kv8::PR_KEYS + 1;
+        if (items * H_kv > INT32_MAX / 2 / tiles) return LSE_ERR_UNSUPPORTED;
+    }
     if (!aligned(q, 16) || !aligned(o, 16) || q_stride_h % 8 || q_stride_m % 8 || o_stride_h % 8 || o_stride_m % 8 ||
         !aligned(context_len, 4) || !aligned(query_offset, 4) || !aligned(q_start, 4) || !aligned(q_len, 4))
         return LSE_ERR_ALIGNMENT;

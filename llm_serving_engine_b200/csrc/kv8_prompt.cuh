@@ -24,6 +24,8 @@
 // average) they are dealt whole instead: a joint costs more than it gains there.
 #pragma once
 
+#include <climits>
+
 #include "common.cuh"
 #include "kv8_attn.cuh"
 #include "kv8_decode.cuh"
@@ -54,47 +56,52 @@ struct PromptSmem {
     static constexpr int BYTES = TABLE + PR_TABLES * (PR_KEYS * 8 + 32) + 1024;  // + alignment
 };
 
+__device__ __forceinline__ int64_t floor_div(int64_t a, int64_t b) { return a / b; }
+
 // What a CTA does next: position tiles [j0, j1) of item i of (entry e, KV head kvh).
 struct PromptSegment {
     int e, kvh, i, j0, j1, tiles;
     int q_start, q_len, offset, context;
-    int64_t item;  // split: the item's first tile
+    int item;  // split: the item's first tile
 };
 
 // The schedule, the same in every role; see the header comment.  Each warp keeps a copy in shared
 // memory (its fields would be registers that the softmax has no room for).
 struct PromptSchedule {
-    int tok;            // tokens per item
-    int64_t at, end, total, active;  // split: this CTA's run of tiles; whole: its next item and their number
-    bool split;
+    int tok;                     // tokens per item
+    int at, end, total, active;  // split: this CTA's run of tiles; whole: its next item and their number
+    int split;
     int e, kvh, i;
-    int64_t first;      // split: first tile of the current item; whole: first item of entry e
+    int first;                   // split: first tile of the current item; whole: first item of entry e
     int q_start, q_len, offset, context, nq;
 
-    __device__ __forceinline__ static int context_of(const AttnParams &p, int e) {
-        const int64_t most = static_cast<int64_t>(p.bt_cols) * p.block_size;
-        return static_cast<int>(min(static_cast<int64_t>(max(__ldcg(p.context_len + e), 0)), most));
-    }
     __device__ __forceinline__ static int tiles_of(int context, int offset, int q_len, int tok, int i) {
-        const int64_t seen = min(static_cast<int64_t>(context), static_cast<int64_t>(offset) + min(q_len, (i + 1) * tok));
-        return static_cast<int>(max(static_cast<int64_t>(1), (seen + PR_KEYS - 1) / PR_KEYS));
+        const int seen = min(context, offset + min(q_len, (i + 1) * tok));
+        return max(1, (seen + PR_KEYS - 1) >> 7);
     }
     __device__ __forceinline__ void load_entry(const AttnParams &p) {
+        q_len = offset = context = q_start = nq = 0;
         if (e >= p.E) return;
         q_start = __ldcg(p.q_start + e);
         q_len = max(__ldcg(p.q_len + e), 0);
         offset = __ldcg(p.query_offset + e);
-        context = context_of(p, e);
+        context = min(max(__ldcg(p.context_len + e), 0), p.bt_cols * p.block_size);
         nq = (q_len + tok - 1) / tok;
+    }
+    // Tiles of entry e for one KV head (its fields loaded).
+    __device__ __forceinline__ int entry_tiles() const {
+        int n = 0;
+#pragma unroll 1
+        for (int k = 0; k < nq; ++k) n += tiles_of(context, offset, q_len, tok, k);
+        return n;
     }
     __device__ __forceinline__ bool next(const AttnParams &p, PromptSegment &s) {
         if (at >= end) return false;
         if (split) {
             const int n = tiles_of(context, offset, q_len, tok, i);
-            s.j0 = static_cast<int>(at - first);
-            s.j1 = static_cast<int>(min(end, first + n) - first);
+            s.j0 = at - first;
+            s.j1 = min(end, first + n) - first;
             fill(s, n);
-            s.item = first;
             at = first + s.j1;
             if (s.j1 == n) {  // the next item
                 first += n;
@@ -110,12 +117,12 @@ struct PromptSchedule {
                 }
             }
         } else {
-            while (at >= first + static_cast<int64_t>(nq) * p.H_kv) {
-                first += static_cast<int64_t>(nq) * p.H_kv;
+            while (at >= first + nq * p.H_kv) {
+                first += nq * p.H_kv;
                 ++e;
                 load_entry(p);
             }
-            const int k = static_cast<int>(at - first);
+            const int k = at - first;
             kvh = k % p.H_kv;
             i = nq - 1 - k / p.H_kv;  // the longest first
             s.j0 = 0;
@@ -134,9 +141,12 @@ struct PromptSchedule {
         s.q_len = q_len;
         s.offset = offset;
         s.context = context;
+        s.item = first;
     }
     // CTA whose run holds a tile (split)
-    __device__ __forceinline__ int cta_of(int64_t tile) const { return static_cast<int>(((tile + 1) * active - 1) / total); }
+    __device__ __forceinline__ int cta_of(int tile) const {
+        return static_cast<int>(floor_div(static_cast<int64_t>(tile + 1) * active - 1, total));
+    }
 };
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -197,8 +207,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
     __shared__ __align__(8) uint64_t s_bar[BARS];
     __shared__ uint32_t s_tmem, s_rows[2][PR_KEYS];
     __shared__ int s_abort_word, s_last;
-    __shared__ int64_t s_sum[PR_WARPS][2];
-    __shared__ int64_t s_found[3];
+    __shared__ int s_sum[PR_WARPS], s_found[3];
     __shared__ PromptSchedule s_sched[PR_WARPS];
     __shared__ PromptSegment s_seg[PR_WARPS][2];
     const uint32_t base = (ptx::smem_u32(s_raw) + 1023u) & ~1023u;
@@ -248,99 +257,80 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
         warp_wait(b, phase);
     };
 
-    // ---- the schedule ------------------------------------------------------------------------------
+    // ---- the schedule (all counts fit 32 bits: the host bounds them) ---------------------------------
     const int item_tokens = PR_ROWS >> log_g;
     {
-        PromptSchedule sched;
+        PromptSchedule sched{};
         sched.tok = item_tokens;
-        auto entry = [&](int e, int64_t &tiles, int64_t &items) {
-            tiles = items = 0;
-            if (e >= p.E) return;
-            const int len = max(__ldcg(p.q_len + e), 0), off = __ldcg(p.query_offset + e);
-            const int ctx = PromptSchedule::context_of(p, e);
-            items = (len + sched.tok - 1) / sched.tok;
-            for (int i = 0; i < items; ++i) tiles += PromptSchedule::tiles_of(ctx, off, len, sched.tok, i);
-        };
-        int64_t tiles_all = 0, items_all = 0;
-        for (int e0 = 0; e0 < p.E; e0 += PR_THREADS) {
-            int64_t tiles, items;
-            const int e = e0 + threadIdx.x;
-            entry(e, tiles, items);
-            if (blockIdx.x == 0 && e < p.E && items > 0) {
-                const int start = __ldcg(p.q_start + e), len = __ldcg(p.q_len + e);
-                const int64_t seen = min(static_cast<int64_t>(__ldcg(p.context_len + e)), static_cast<int64_t>(__ldcg(p.query_offset + e)) + len);
-                if (start < 0 || start > p.tokens - len || seen > static_cast<int64_t>(p.bt_cols) * p.block_size)
-                    report_status(LSE_ERR_INVALID_ARG);
-            }
-#pragma unroll
-            for (int k = 16; k > 0; k >>= 1) {
-                tiles += __shfl_xor_sync(0xffffffffu, tiles, k);
-                items += __shfl_xor_sync(0xffffffffu, items, k);
-            }
-            if (lane == 0) {
-                s_sum[warp][0] = tiles;
-                s_sum[warp][1] = items;
-            }
-            __syncthreads();
-            for (int i = 0; i < PR_WARPS; ++i) {
-                tiles_all += s_sum[i][0];
-                items_all += s_sum[i][1];
-            }
-            __syncthreads();
-        }
-        tiles_all *= p.H_kv;
-        items_all *= p.H_kv;
-        sched.split = tiles_all >= PR_SPLIT_TILES * items_all;
-        sched.total = tiles_all;
-        sched.e = -1;
-        sched.kvh = sched.i = 0;
-        sched.first = 0;
-        sched.nq = 0;
-        if (sched.split) {
-            // no run shorter than SPLIT_TILES tiles
-            sched.active = max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), tiles_all / PR_SPLIT_TILES));
-            const bool in = static_cast<int64_t>(blockIdx.x) < sched.active;
-            sched.at = in ? blockIdx.x * tiles_all / sched.active : 0;
-            sched.end = in ? (blockIdx.x + 1) * tiles_all / sched.active : 0;
-            // the entry that tile `at` belongs to
-            if (threadIdx.x == 0) s_found[0] = -1;
-            int64_t before_all = 0;
+        // Entry e0 + threadIdx.x of a round: its tiles, and by `incl` the running sum over the round.
+        int tiles_all = 0, items_all = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {  // the totals, then the entry that this CTA starts in
+            int base_tiles = 0, items = 0;
+#pragma unroll 1
             for (int e0 = 0; e0 < p.E; e0 += PR_THREADS) {
-                int64_t tiles, items;
-                entry(e0 + threadIdx.x, tiles, items);
-                int64_t incl = tiles;
+                sched.e = e0 + threadIdx.x;
+                sched.load_entry(p);
+                const int tiles = sched.entry_tiles();
+                if (pass == 0 && blockIdx.x == 0 && sched.nq > 0 &&
+                    (sched.q_start < 0 || sched.q_start > p.tokens - sched.q_len ||
+                     min(__ldcg(p.context_len + sched.e), sched.offset + sched.q_len) > p.bt_cols * p.block_size))
+                    report_status(LSE_ERR_INVALID_ARG);
+                items += __reduce_add_sync(0xffffffffu, sched.nq);
+                int incl = tiles;
 #pragma unroll
                 for (int k = 1; k < 32; k <<= 1) {
-                    const int64_t v = __shfl_up_sync(0xffffffffu, incl, k);
+                    const int v = __shfl_up_sync(0xffffffffu, incl, k);
                     if (lane >= k) incl += v;
                 }
-                if (lane == 31) s_sum[warp][0] = incl;
+                if (lane == 31) s_sum[warp] = incl;
                 __syncthreads();
-                int64_t before = before_all + incl - tiles;
+                int before = base_tiles + incl - tiles;
+#pragma unroll 1
                 for (int i = 0; i < PR_WARPS; ++i) {
-                    if (i < warp) before += s_sum[i][0];
-                    before_all += s_sum[i][0];
+                    if (i < warp) before += s_sum[i];
+                    base_tiles += s_sum[i];
                 }
-                if (tiles > 0 && sched.at >= before * p.H_kv && sched.at < (before + tiles) * p.H_kv) {
-                    s_found[0] = e0 + threadIdx.x;
+                if (pass == 1 && tiles > 0 && sched.at >= before * p.H_kv && sched.at < (before + tiles) * p.H_kv) {
+                    s_found[0] = sched.e;
                     s_found[1] = before * p.H_kv;
                     s_found[2] = tiles;
                 }
                 __syncthreads();
             }
-            if (sched.at < sched.end) {
-                sched.e = static_cast<int>(s_found[0]);
-                sched.load_entry(p);
-                const int64_t off = sched.at - s_found[1];
-                sched.kvh = static_cast<int>(off / s_found[2]);
-                sched.first = s_found[1] + sched.kvh * s_found[2];
-                for (int n; sched.first + (n = PromptSchedule::tiles_of(sched.context, sched.offset, sched.q_len, sched.tok, sched.i)) <= sched.at; ++sched.i)
-                    sched.first += n;
+            if (pass == 1) break;
+            if (lane == 0) s_sum[warp] = items;
+            __syncthreads();
+#pragma unroll 1
+            for (int i = 0; i < PR_WARPS; ++i) items_all += s_sum[i];
+            __syncthreads();
+            items_all *= p.H_kv;
+            tiles_all = base_tiles * p.H_kv;
+            sched.split = tiles_all >= PR_SPLIT_TILES * items_all;
+            sched.total = tiles_all;
+            if (!sched.split) break;
+            // no run shorter than SPLIT_TILES tiles
+            sched.active = max(1, min(static_cast<int>(gridDim.x), tiles_all / PR_SPLIT_TILES));
+            sched.at = sched.end = 0;
+            if (static_cast<int>(blockIdx.x) < sched.active) {
+                sched.at = static_cast<int>(floor_div(static_cast<int64_t>(blockIdx.x) * tiles_all, sched.active));
+                sched.end = static_cast<int>(floor_div(static_cast<int64_t>(blockIdx.x + 1) * tiles_all, sched.active));
             }
-        } else {
+        }
+        if (!sched.split) {
             sched.active = gridDim.x;
             sched.at = blockIdx.x;
             sched.end = items_all;
+            sched.e = -1;
+            sched.first = sched.nq = 0;
+        } else if (sched.at < sched.end) {
+            sched.e = s_found[0];
+            sched.load_entry(p);
+            sched.kvh = (sched.at - s_found[1]) / s_found[2];
+            sched.first = s_found[1] + sched.kvh * s_found[2];
+#pragma unroll 1
+            for (int n; sched.first + (n = PromptSchedule::tiles_of(sched.context, sched.offset, sched.q_len, sched.tok, sched.i)) <= sched.at; ++sched.i)
+                sched.first += n;
         }
         if (lane == 0) s_sched[warp] = sched;
     }
@@ -416,7 +406,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             const int r = 128 * t + row, in = s.i * item_tokens + (r >> log_g);
             const int tok = s.q_start + in;
             const bool live = in < s.q_len && tok >= 0 && tok < p.tokens;
-            const int limit = live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(s.context), static_cast<int64_t>(s.offset) + in + 1))) : 0;
+            // positions below `limit` are seen; what a row that is not stored sees does not matter
+            const int limit = live ? max(0, min(s.context, s.offset + in + 1)) : INT_MAX / 2;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const float c = p.scale_log2 * back;
             float M = M_NONE;
@@ -631,7 +622,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             const PromptSegment &s = s_seg[warp][seg_n & 1];
             const int pos = j * PR_KEYS + me;
             // positions that some row of the item sees
-            const int64_t seen = min(static_cast<int64_t>(s.context), static_cast<int64_t>(s.offset) + min(s.q_len, (s.i + 1) * item_tokens));
+            const int seen = min(s.context, s.offset + min(s.q_len, (s.i + 1) * item_tokens));
             kvh = s.kvh;
             if (pos < seen) {
                 const int page = pos / p.block_size;
