@@ -45,9 +45,27 @@ extern "C" int lse_token_logprobs(const void *logits, int dtype, int64_t M, int6
     p.M = static_cast<int>(M);
     p.V = static_cast<int>(V);
     p.k = static_cast<int>(top_k);
+    // CTAs of a row: enough to give every SM a few, as long as each of a CTA's warps has a group
+    const int step = 64 * static_cast<int>(16 / el);  // logits of one warp's loads
+    p.group = step;
+    p.cluster = 1;
+    while (p.cluster < logprobs::MAX_CLUSTER && M * p.cluster < 4 * host::num_sms(dev) &&
+           V > static_cast<int64_t>(p.cluster) * 2 * logprobs::WARPS * step)
+        p.cluster *= 2;
+    const int limit = p.cluster > 1 ? 256 : logprobs::MAX_GROUPS;
+    auto groups = [&] { return (V + 16 + static_cast<int64_t>(p.group) * p.cluster - 1) / (static_cast<int64_t>(p.group) * p.cluster); };
+    while (groups() > limit) p.group *= 2;
+    p.groups = static_cast<int>(groups());
+    p.fine = p.cluster == 1 && p.group == step && p.groups * 64 <= logprobs::MAX_GROUPS;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(M)), dim3(logprobs::THREADS), 0, static_cast<cudaStream_t>(stream));
+    cudaLaunchAttribute pdl[1], attr[2];
+    if (M * p.cluster > INT32_MAX) return LSE_ERR_UNSUPPORTED;
+    host::launch_config(cfg, pdl, dim3(static_cast<unsigned>(M * p.cluster)), dim3(logprobs::THREADS), 0, static_cast<cudaStream_t>(stream));
+    attr[0] = pdl[0];
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {static_cast<unsigned>(p.cluster), 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = p.cluster > 1 ? 2 : 1;
     const auto kernel = dtype == LSE_F32 ? logprobs::rows_kernel<float>
                         : dtype == LSE_F16 ? logprobs::rows_kernel<__half> : logprobs::rows_kernel<__nv_bfloat16>;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
