@@ -410,12 +410,13 @@ int lse_kv8_rope_append(const void *qkv, int dtype, int64_t M, int64_t ld_qkv, i
                         int64_t E, void *stream);
 
 /*
- * Values of the pages block_ids[0 .. n) (int64) of one pool: out [n, H_kv, block_size, D] of
+ * Values of the pages block_ids[0 .. n) (int64): k_out and v_out [n, H_kv, block_size, D] of
  * `dtype` (LSE_BF16 or LSE_F16), contiguous, 16-byte aligned, code * scale rounded once.  An id
- * outside [0, num_blocks) gives zeros and LSE_ERR_INVALID_ARG in lse_device_status.
+ * outside [0, num_blocks) gives zeros and LSE_ERR_INVALID_ARG in lse_device_status.  D a multiple of 16.
  */
-int lse_kv8_read(const int8_t *pool, const float *scale, int64_t num_blocks, int64_t block_size, int64_t H_kv, int64_t D,
-                 const int64_t *block_ids, int64_t n, void *out, int dtype, void *stream);
+int lse_kv8_read(const int8_t *k_pool, const int8_t *v_pool, const float *k_scale, const float *v_scale, int64_t num_blocks,
+                 int64_t block_size, int64_t H_kv, int64_t D, const int64_t *block_ids, int64_t n, void *k_out, void *v_out,
+                 int dtype, void *stream);
 
 /*
  * Decode attention over the 8-bit cache, one query token per entry:

@@ -86,7 +86,7 @@ SIGNATURES = {
                              _I64, _I64, ctypes.c_float, _P, _I64, _I64, _P], _I32),
     "lse_kv8_rope_append": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I32, _I64, _I32, _P, _P, _P, _P, _P,
                              _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P], _I32),
-    "lse_kv8_read": ([_P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I32, _P], _I32),
+    "lse_kv8_read": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _I32, _P], _I32),
     "lse_kv8_decode_attention_workspace": ([_I64, _I64, _I64], _SZ),
     "lse_kv8_decode_attention": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64,
                                   _I64, _P, ctypes.c_float, _P, _I64, _I64, _P, _SZ, _P], _I32),

@@ -57,13 +57,25 @@ int finish(cudaError_t e, const char *where) {
 
 template <typename T>
 int launch_append(kv8::AppendParams<T> &p, int sms, cudaStream_t st) {
-    const int64_t q_elems = static_cast<int64_t>(p.M) * p.H * p.D;
-    p.q_blocks = static_cast<int>(std::min<int64_t>((q_elems + kv8::APPEND_THREADS - 1) / kv8::APPEND_THREADS, 8LL * sms));
     // an entry of n tokens touches at most n / block_size + 2 pages (fewer warps only loop more)
     const int64_t pages = static_cast<int64_t>(p.M) / p.block_size + 2LL * p.E;
     const int64_t kv = std::min<int64_t>((pages * p.H_kv * 2 + 7) / 8, 8LL * sms);
+    // vectors: both runs of a lane rotate together, and the tables' rows are 16-byte aligned
+    const int cs = p.cs_type == 0 ? 4 : 2;
+    const bool vec = p.R == 0 || (p.R % (p.interleaved ? 8 : 16) == 0 && aligned(p.cos, 16) && aligned(p.sin, 16) && p.ld_cs * cs % 16 == 0);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
+    if (vec) {
+        // a warp takes 16 heads of a token where that still gives each SM 32 warps, else one load's worth
+        const int64_t few = 512 / p.D;
+        const int heads = static_cast<int>(static_cast<int64_t>(p.M) * p.H / kv8::Q_HEADS >= 32LL * sms ? kv8::Q_HEADS : few);
+        p.q_blocks = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.M) * ((p.H + heads - 1) / heads) + 7) / 8, 16LL * sms));
+        host::launch_config(cfg, attr, dim3(static_cast<unsigned>(p.q_blocks + kv)), dim3(kv8::APPEND_THREADS), 0, st);
+        return finish(cudaLaunchKernelEx(&cfg, p.D == 128 ? kv8::append_vec_kernel<T, 128> : kv8::append_vec_kernel<T, 64>, p, heads),
+                      "kv8_rope_append launch");
+    }
+    const int64_t q_elems = static_cast<int64_t>(p.M) * p.H * p.D;
+    p.q_blocks = static_cast<int>(std::min<int64_t>((q_elems + kv8::APPEND_THREADS - 1) / kv8::APPEND_THREADS, 8LL * sms));
     host::launch_config(cfg, attr, dim3(static_cast<unsigned>(p.q_blocks + kv)), dim3(kv8::APPEND_THREADS), 0, st);
     return finish(cudaLaunchKernelEx(&cfg, kv8::append_kernel<T>, p), "kv8_rope_append launch");
 }
@@ -188,27 +200,31 @@ int lse_kv8_rope_append(const void *qkv, int dtype, int64_t M, int64_t ld_qkv, i
                host::num_sms(dev), static_cast<cudaStream_t>(stream));
 }
 
-int lse_kv8_read(const int8_t *pool, const float *scale, int64_t num_blocks, int64_t block_size, int64_t H_kv, int64_t D,
-                 const int64_t *block_ids, int64_t n, void *out, int dtype, void *stream) {
+int lse_kv8_read(const int8_t *k_pool, const int8_t *v_pool, const float *k_scale, const float *v_scale, int64_t num_blocks,
+                 int64_t block_size, int64_t H_kv, int64_t D, const int64_t *block_ids, int64_t n, void *k_out, void *v_out,
+                 int dtype, void *stream) {
     if (num_blocks <= 0 || block_size <= 0 || H_kv <= 0 || D <= 0 || n < 0) return LSE_ERR_INVALID_ARG;
     if (dtype != LSE_BF16 && dtype != LSE_F16) return LSE_ERR_UNSUPPORTED;
     if (n == 0) return LSE_OK;
-    if (!pool || !scale || !block_ids || !out) return LSE_ERR_INVALID_ARG;
+    if (!k_pool || !v_pool || !k_scale || !v_scale || !block_ids || !k_out || !v_out) return LSE_ERR_INVALID_ARG;
     if (num_blocks > INT32_MAX / 2 || block_size * D > INT32_MAX / 2 || H_kv > 65535 || n > INT32_MAX / 2 || D % 16)
         return LSE_ERR_UNSUPPORTED;
-    if (!aligned(pool, 16) || !aligned(out, 16) || !aligned(scale, 4) || !aligned(block_ids, 8)) return LSE_ERR_ALIGNMENT;
+    if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(k_scale, 4) ||
+        !aligned(v_scale, 4) || !aligned(block_ids, 8))
+        return LSE_ERR_ALIGNMENT;
     int dev = 0;
     if (int rc = host::current_device(&dev)) return rc;
-    const int64_t total = n * H_kv * block_size * D;
-    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16LL * host::num_sms(dev));
+    const int64_t vecs = block_size * D / 16, total = n * H_kv * vecs;
+    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 8LL * host::num_sms(dev));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<cudaStream_t>(stream));
-    const int nb = static_cast<int>(num_blocks), hk = static_cast<int>(H_kv), pe = static_cast<int>(block_size * D);
+    host::launch_config(cfg, attr, dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, static_cast<cudaStream_t>(stream));
+    const int nb = static_cast<int>(num_blocks), hk = static_cast<int>(H_kv), pv = static_cast<int>(vecs);
     const cudaError_t e = dtype == LSE_F16
-        ? cudaLaunchKernelEx(&cfg, kv8::read_kernel<__half>, pool, scale, nb, hk, pe, block_ids, n, static_cast<__half *>(out))
-        : cudaLaunchKernelEx(&cfg, kv8::read_kernel<__nv_bfloat16>, pool, scale, nb, hk, pe, block_ids, n,
-                             static_cast<__nv_bfloat16 *>(out));
+        ? cudaLaunchKernelEx(&cfg, kv8::read_kernel<__half>, k_pool, v_pool, k_scale, v_scale, nb, hk, pv, block_ids, n,
+                             static_cast<__half *>(k_out), static_cast<__half *>(v_out))
+        : cudaLaunchKernelEx(&cfg, kv8::read_kernel<__nv_bfloat16>, k_pool, v_pool, k_scale, v_scale, nb, hk, pv, block_ids, n,
+                             static_cast<__nv_bfloat16 *>(k_out), static_cast<__nv_bfloat16 *>(v_out));
     return finish(e, "kv8_read launch");
 }
 

@@ -14,9 +14,15 @@
 //     half:        partner(d) = d + R/2 (sign -) for d < R/2, d - R/2 (sign +) above
 //     interleaved: partner(d) = d + 1 (sign -) for even d, d - 1 (sign +) for odd d
 //
-// One warp per (page, KV head, k or v): it owns the page's scale, so no atomics.  Bound by
-// latency for decode (one row per page) and by DRAM for prompts.
+// One warp per (page, KV head, k or v): it owns the page's scale, so no atomics, and goes over the
+// page's new rows twice (their maximum, then the codes; up to one row a lane group, which is every
+// decode step, the second time from registers).  q in warps of their own, a token's heads a few at a
+// time with its cos and sin in registers.  A lane holds two 16-byte runs of a row, a pair's
+// two sides, so that all loads and stores are vectors.  Bound by DRAM for prompts, by latency
+// for decode (one row per page).
 #pragma once
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -64,6 +70,57 @@ __device__ __forceinline__ float rotated(const AppendParams<T> &p, const T *x, i
     return a * cs + (first ? -b : b) * sn;
 }
 
+// Running sums, over the entries of a round, of the pages that each touches; returns the round's total.
+template <typename T>
+__device__ __forceinline__ int scan_pages(const AppendParams<T> &p, int e0, int *s_pages, int *s_warp) {
+    const int e = e0 + threadIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int n = 0;
+    if (e < p.E) {
+        const int len = p.q_len[e], off = p.query_offset[e];
+        if (len > 0 && off >= 0) n = (off + len - 1) / p.block_size - off / p.block_size + 1;
+    }
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, n, k);
+        if (lane >= k) n += v;
+    }
+    if (lane == 31) s_warp[warp] = n;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) n += s_warp[w];
+    s_pages[threadIdx.x] = n;
+    __syncthreads();
+    return s_pages[APPEND_THREADS - 1];
+}
+
+// One page of one entry: its block and the new positions [first, last) that it takes.
+struct PageItem {
+    int off, row0, first, last, old, blk;
+
+    // The pg-th page of the round; false (and reported) where it or its rows do not exist.
+    template <typename T>
+    __device__ __forceinline__ bool find(const AppendParams<T> &p, int e0, const int *s_pages, int pg, int lane) {
+        int lo = 0, hi = APPEND_THREADS - 1;  // the first entry whose running sum exceeds pg
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (s_pages[mid] > pg) hi = mid;
+            else lo = mid + 1;
+        }
+        const int e = e0 + lo;
+        const int len = p.q_len[e];
+        off = p.query_offset[e];
+        row0 = p.q_start[e];
+        const int page = off / p.block_size + pg - (lo ? s_pages[lo - 1] : 0);
+        first = max(off, page * p.block_size);
+        last = min(off + len, (page + 1) * p.block_size);
+        old = first - page * p.block_size;
+        blk = page < p.bt_cols ? p.block_table[e * p.bt_stride + page] : -1;
+        if (blk >= 0 && blk < p.num_blocks && row0 >= 0 && row0 <= p.M - (last - off)) return true;
+        if (lane == 0) report_status(LSE_ERR_INVALID_ARG);
+        return false;
+    }
+};
+
+// The general form, for rotations that do not fall on vectors: an element at a time.
 template <typename T>
 __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendParams<T> p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -81,49 +138,17 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
         }
         return;
     }
-    __shared__ int s_pages[APPEND_THREADS];  // running sum of the pages that each entry touches
+    __shared__ int s_pages[APPEND_THREADS], s_warp[APPEND_THREADS / 32];
     const int warps = (gridDim.x - p.q_blocks) * (APPEND_THREADS / 32);
     const int me = (blockIdx.x - p.q_blocks) * (APPEND_THREADS / 32) + warp;
     for (int e0 = 0; e0 < p.E; e0 += APPEND_THREADS) {
-        __syncthreads();
-        {
-            const int e = e0 + threadIdx.x;
-            int n = 0;
-            if (e < p.E) {
-                const int len = p.q_len[e], off = p.query_offset[e];
-                if (len > 0 && off >= 0) n = (off + len - 1) / p.block_size - off / p.block_size + 1;
-            }
-            s_pages[threadIdx.x] = n;
-            __syncthreads();
-            for (int k = 1; k < APPEND_THREADS; k <<= 1) {
-                const int v = static_cast<int>(threadIdx.x) >= k ? s_pages[threadIdx.x - k] : 0;
-                __syncthreads();
-                s_pages[threadIdx.x] += v;
-                __syncthreads();
-            }
-        }
-        const int64_t items = static_cast<int64_t>(s_pages[APPEND_THREADS - 1]) * p.H_kv * 2;
-        for (int64_t it = me; it < items; it += warps) {
-            const int which = static_cast<int>(it & 1);
-            const int h = static_cast<int>((it >> 1) % p.H_kv);
-            const int pg = static_cast<int>((it >> 1) / p.H_kv);
-            int lo = 0, hi = APPEND_THREADS - 1;  // the first entry whose running sum exceeds pg
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (s_pages[mid] > pg) hi = mid;
-                else lo = mid + 1;
-            }
-            const int e = e0 + lo;
-            const int off = p.query_offset[e], len = p.q_len[e], row0 = p.q_start[e];
-            const int page = off / p.block_size + pg - (lo ? s_pages[lo - 1] : 0);
-            const int first = max(off, page * p.block_size);
-            const int last = min(off + len, (page + 1) * p.block_size);  // positions [first, last) are new
-            const int old = first - page * p.block_size;
-            const int blk = page < p.bt_cols ? p.block_table[e * p.bt_stride + page] : -1;
-            if (blk < 0 || blk >= p.num_blocks || row0 < 0 || row0 + (last - off) > p.M) {
-                if (lane == 0) report_status(LSE_ERR_INVALID_ARG);
-                continue;
-            }
+        const int items = scan_pages(p, e0, s_pages, s_warp) * p.H_kv * 2;
+        for (int it = me; it < items; it += warps) {
+            const int which = it & 1, h = (it >> 1) % p.H_kv;
+            PageItem g;
+            if (!g.find(p, e0, s_pages, (it >> 1) / p.H_kv, lane)) continue;
+            const int first = g.first, last = g.last, off = g.off, row0 = g.row0, blk = g.blk, old = g.old;
+            const int page0 = first - old;  // the page's first position
             const T *x0 = p.qkv + static_cast<int64_t>(p.H + which * p.H_kv + h) * p.D;
             float top = 0.f;
             bool bad = false;
@@ -150,7 +175,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
             for (int pos = first; pos < last; ++pos) {
                 const int m = row0 + pos - off;
                 const T *x = x0 + m * p.ld_qkv;
-                int8_t *row = dst + (pos - page * p.block_size) * p.D;
+                int8_t *row = dst + (pos - page0) * p.D;
                 for (int d = lane; d < p.D; d += 32) {
                     const float v = which == 0 ? rotated(p, x, m, d) : to_float(x[d]);
                     float c = 0.f;
@@ -160,26 +185,240 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
             }
             if (lane == 0) p.scale[which][cell] = bad ? __int_as_float(0x7fffffff) : s;
         }
+        __syncthreads();  // s_pages is used again
     }
 }
 
-// Values of the pages ids[0..n): out[i, h, t, d] = code * scale, rounded once to T.
+// ---- the vector form: D / 16 lanes a row, 16 elements each (two runs of 8) -----------------------------
+
+// Two runs of a row as this lane holds them: half: [d, d + 8) and their partners R/2 further on (or two
+// neighbouring runs of the part that does not rotate); interleaved: 16 neighbours.
+template <typename T, int D>
+struct Lane {
+    int d0, d1;      // where the runs start
+    bool r0, r1;     // whether they rotate
+    float c[16], s[16];  // their cos and sin
+
+    __device__ __forceinline__ Lane(const AppendParams<T> &p, int sub) {
+        if (p.interleaved) {
+            d0 = 16 * sub;
+            d1 = d0 + 8;
+            r0 = d0 < p.R;
+            r1 = d1 < p.R;
+        } else {
+            r0 = r1 = 16 * sub < p.R;
+            d0 = r0 ? 8 * sub : 16 * sub;
+            d1 = r0 ? d0 + p.R / 2 : d0 + 8;
+        }
+    }
+    // 8 table values from element i (16-byte aligned rows)
+    __device__ __forceinline__ static void table8(float (&v)[16], int at, const void *t, int type, int64_t i) {
+        if (type == 0) {
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(t) + i));
+            const float4 b = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(t) + i) + 1);
+            v[at] = a.x; v[at + 1] = a.y; v[at + 2] = a.z; v[at + 3] = a.w;
+            v[at + 4] = b.x; v[at + 5] = b.y; v[at + 6] = b.z; v[at + 7] = b.w;
+        } else {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(t) + i));
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint16_t h = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+                v[at + k] = type == 1 ? __uint_as_float(static_cast<uint32_t>(h) << 16) : __half2float(__ushort_as_half(h));
+            }
+        }
+    }
+    __device__ __forceinline__ void tables(const AppendParams<T> &p, int m) {
+        const int64_t row = m * p.ld_cs;
+        if (r0) {
+            table8(c, 0, p.cos, p.cs_type, row + d0);
+            table8(s, 0, p.sin, p.cs_type, row + d0);
+        }
+        if (r1) {
+            table8(c, 8, p.cos, p.cs_type, row + d1);
+            table8(s, 8, p.sin, p.cs_type, row + d1);
+        }
+    }
+    __device__ __forceinline__ void load(float (&v)[16], const T *x) const {
+        const uint4 a = *reinterpret_cast<const uint4 *>(x + d0), b = *reinterpret_cast<const uint4 *>(x + d1);
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float2 f;
+            if constexpr (std::is_same_v<T, __half>) f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+            else f = bf16x2_to_f32x2(w[k]);
+            v[2 * k] = f.x;
+            v[2 * k + 1] = f.y;
+        }
+    }
+    __device__ __forceinline__ void turn(float (&v)[16], bool interleaved) const {
+        if (interleaved) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 2)
+                if (k < 8 ? r0 : r1) {
+                    const float a = v[k], b = v[k + 1];
+                    v[k] = a * c[k] + -b * s[k];
+                    v[k + 1] = b * c[k + 1] + a * s[k + 1];
+                }
+        } else if (r0) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float a = v[k], b = v[k + 8];
+                v[k] = a * c[k] + -b * s[k];
+                v[k + 8] = b * c[k + 8] + a * s[k + 8];
+            }
+        }
+    }
+};
+
+constexpr int Q_HEADS = 16;  // q heads that a warp takes of a token (fewer where there are few tokens)
+
+template <typename T, int D>
+__global__ void __launch_bounds__(APPEND_THREADS) append_vec_kernel(const AppendParams<T> p, const int q_heads) {
+    constexpr int LANES = D / 16, ROWS = 32 / LANES;  // lanes of a row, rows of a warp
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // qkv is the previous kernel's output
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int sub = lane % LANES, part = lane / LANES;
+    Lane<T, D> my(p, sub);
+    if (static_cast<int>(blockIdx.x) < p.q_blocks) {
+        const int blocks = (p.H + q_heads - 1) / q_heads;
+        const int64_t items = static_cast<int64_t>(p.M) * blocks;
+        for (int64_t it = blockIdx.x * static_cast<int64_t>(APPEND_THREADS / 32) + warp; it < items;
+             it += static_cast<int64_t>(p.q_blocks) * (APPEND_THREADS / 32)) {
+            const int m = static_cast<int>(it / blocks), h0 = static_cast<int>(it % blocks) * q_heads;
+            my.tables(p, m);
+#pragma unroll 2
+            for (int h = h0 + part; h < min(h0 + q_heads, p.H); h += ROWS) {
+                float v[16];
+                my.load(v, p.qkv + m * p.ld_qkv + static_cast<int64_t>(h) * D);
+                my.turn(v, p.interleaved);
+                T *o = p.q_out + (static_cast<int64_t>(h) * p.M + m) * D;
+                uint32_t w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if constexpr (std::is_same_v<T, __half>) {
+                        const __half2 x = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+                        w[k] = *reinterpret_cast<const uint32_t *>(&x);
+                    } else {
+                        const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+                        w[k] = *reinterpret_cast<const uint32_t *>(&x);
+                    }
+                }
+                *reinterpret_cast<uint4 *>(o + my.d0) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4 *>(o + my.d1) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+        }
+        return;
+    }
+    __shared__ int s_pages[APPEND_THREADS], s_warp[APPEND_THREADS / 32];
+    const int warps = (gridDim.x - p.q_blocks) * (APPEND_THREADS / 32);
+    const int me = (blockIdx.x - p.q_blocks) * (APPEND_THREADS / 32) + warp;
+    for (int e0 = 0; e0 < p.E; e0 += APPEND_THREADS) {
+        const int items = scan_pages(p, e0, s_pages, s_warp) * p.H_kv * 2;
+        for (int it = me; it < items; it += warps) {
+            const int which = it & 1, h = (it >> 1) % p.H_kv;
+            PageItem g;
+            if (!g.find(p, e0, s_pages, (it >> 1) / p.H_kv, lane)) continue;
+            const int rows = g.last - g.first;
+            const T *x = p.qkv + (g.row0 + g.first - g.off) * p.ld_qkv + static_cast<int64_t>(p.H + which * p.H_kv + h) * D;
+            const int m0 = g.row0 + g.first - g.off;
+            const int64_t cell = static_cast<int64_t>(g.blk) * p.H_kv + h;
+            int8_t *dst = p.pool[which] + (cell * p.block_size + g.old) * D;  // the first new row
+            const float s_old = g.old > 0 ? __ldcg(p.scale[which] + cell) : 0.f;
+            // this lane's part of row r, as it will be quantised
+            auto value = [&](float (&v)[16], int r) {
+                my.load(v, x + r * p.ld_qkv);
+                if (which == 0) {
+                    my.tables(p, m0 + r);
+                    my.turn(v, p.interleaved);
+                }
+            };
+            float v[16];
+            float top = 0.f;
+            bool bad = s_old != s_old;
+            for (int r = part; r < rows; r += ROWS) {
+                value(v, r);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    bad |= !(fabsf(v[k]) <= 3.402823466e38f);
+                    top = fmaxf(top, fabsf(v[k]));
+                }
+            }
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+            bad = __any_sync(0xffffffffu, bad);
+            const float s = fmaxf(s_old, __fdiv_rn(top, 127.f));
+            if (!bad && g.old > 0 && s > s_old) {  // the page's earlier tokens move to the larger scale
+                const float f = __fdiv_rn(s_old, s);
+                uint32_t *c = reinterpret_cast<uint32_t *>(dst - g.old * D);
+                for (int i = lane; i < g.old * D / 4; i += 32) {
+                    const uint32_t u = c[i];
+                    uint32_t o = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        o |= (static_cast<uint32_t>(__float2int_rn(static_cast<float>(static_cast<int8_t>(u >> (8 * k))) * f)) & 0xffu) << (8 * k);
+                    c[i] = o;
+                }
+            }
+            for (int r = part; r < rows; r += ROWS) {
+                if (rows > ROWS) value(v, r);
+                uint32_t o[4] = {0, 0, 0, 0};
+                if (!bad && s > 0.f)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int q = __float2int_rn(fminf(fmaxf(__fdiv_rn(v[k], s), -127.f), 127.f));
+                        o[k / 4] |= (static_cast<uint32_t>(q) & 0xffu) << (8 * (k & 3));
+                    }
+                *reinterpret_cast<uint2 *>(dst + r * D + my.d0) = make_uint2(o[0], o[1]);
+                *reinterpret_cast<uint2 *>(dst + r * D + my.d1) = make_uint2(o[2], o[3]);
+            }
+            if (lane == 0) p.scale[which][cell] = bad ? __int_as_float(0x7fffffff) : s;
+        }
+        __syncthreads();  // s_pages is used again
+    }
+}
+
+// Values of the pages ids[0..n): out[i, h, t, d] = code * scale, rounded once to T; 16 a thread, k and v
+// pools by blockIdx.y.
 template <typename T>
-__global__ void __launch_bounds__(256) read_kernel(const int8_t *pool, const float *scale, int num_blocks, int H_kv,
-                                                   int page_elems, const int64_t *ids, int64_t n, T *out) {
+__global__ void __launch_bounds__(256) read_kernel(const int8_t *k_pool, const int8_t *v_pool, const float *k_scale,
+                                                   const float *v_scale, int num_blocks, int H_kv, int page_vecs,
+                                                   const int64_t *ids, int64_t n, T *k_out, T *v_out) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t total = n * H_kv * page_elems;
+    const int8_t *pool = blockIdx.y ? v_pool : k_pool;
+    const float *scale = blockIdx.y ? v_scale : k_scale;
+    T *out = blockIdx.y ? v_out : k_out;
+    const int64_t total = n * H_kv * page_vecs;
     for (int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x; i < total; i += gridDim.x * static_cast<int64_t>(256)) {
-        const int64_t cell = i / page_elems;
+        const int64_t cell = i / page_vecs;
         const int64_t b = ids[cell / H_kv];
+        uint4 c = make_uint4(0, 0, 0, 0);
+        float s = 0.f;
         if (b < 0 || b >= num_blocks) {
             report_status(LSE_ERR_INVALID_ARG);
-            out[i] = from_float<T>(0.f);
-            continue;
+        } else {
+            const int64_t src = b * H_kv + cell % H_kv;
+            s = __ldcg(scale + src);
+            c = __ldcg(reinterpret_cast<const uint4 *>(pool) + src * page_vecs + i % page_vecs);
         }
-        const int64_t src = b * H_kv + cell % H_kv;
-        out[i] = from_float<T>(static_cast<float>(pool[src * page_elems + i % page_elems]) * scale[src]);
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float a = static_cast<float>(static_cast<int8_t>(w[k / 2] >> (16 * (k & 1)))) * s;
+            const float d = static_cast<float>(static_cast<int8_t>(w[k / 2] >> (16 * (k & 1) + 8))) * s;
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 x = __floats2half2_rn(a, d);
+                o[k] = *reinterpret_cast<const uint32_t *>(&x);
+            } else {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(a, d);
+                o[k] = *reinterpret_cast<const uint32_t *>(&x);
+            }
+        }
+        reinterpret_cast<uint4 *>(out)[2 * i] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4 *>(out)[2 * i + 1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
 }
 

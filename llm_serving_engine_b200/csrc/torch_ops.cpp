@@ -276,12 +276,11 @@ std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor &k, const at::Tenso
     const auto options = k.options().dtype(dtype);
     at::Tensor out[2] = {at::empty({n, c.H_kv(), c.block_size(), c.D()}, options),
                          at::empty({n, c.H_kv(), c.block_size(), c.D()}, options)};
-    const cudaStream_t st = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-    const int dt = dtype == at::kHalf ? LSE_F16 : LSE_BF16;
-    for (int i = 0; i < 2; ++i)
-        check_launch(lse_kv8_read((i ? v : k).data_ptr<int8_t>(), (i ? v_scale : k_scale).data_ptr<float>(), c.num_blocks(),
-                                  c.block_size(), c.H_kv(), c.D(), block_ids.data_ptr<int64_t>(), n, out[i].data_ptr(), dt, st),
-                     "lse_kv8_read");
+    check_launch(lse_kv8_read(k.data_ptr<int8_t>(), v.data_ptr<int8_t>(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
+                              c.num_blocks(), c.block_size(), c.H_kv(), c.D(), block_ids.data_ptr<int64_t>(), n, out[0].data_ptr(),
+                              out[1].data_ptr(), dtype == at::kHalf ? LSE_F16 : LSE_BF16,
+                              at::cuda::getCurrentCUDAStream(dev.index()).stream()),
+                 "lse_kv8_read");
     return {out[0], out[1]};
 }
 

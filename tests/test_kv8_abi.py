@@ -61,7 +61,7 @@ def test_read_and_logprobs_refusals():
     lib = _lib.load()
     bad, off, no = _lib.LSE_ERR_INVALID_ARG, _lib.LSE_ERR_ALIGNMENT, _lib.LSE_ERR_UNSUPPORTED
     read = lambda pool=P, scale=P, nb=4, bs=16, hk=2, D=64, ids=P, n=3, out=P, dt=0: lib.lse_kv8_read(  # noqa: E731
-        pool, scale, nb, bs, hk, D, ids, n, out, dt, None)
+        pool, P, scale, P, nb, bs, hk, D, ids, n, out, P, dt, None)
     assert read(n=0) == _lib.LSE_OK
     for kw in (dict(pool=None), dict(scale=None), dict(ids=None), dict(out=None), dict(nb=0), dict(bs=0), dict(n=-1)):
         assert read(**kw) == bad, kw
