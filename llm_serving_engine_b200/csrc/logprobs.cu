@@ -45,18 +45,18 @@ extern "C" int lse_token_logprobs(const void *logits, int dtype, int64_t M, int6
     p.M = static_cast<int>(M);
     p.V = static_cast<int>(V);
     p.k = static_cast<int>(top_k);
-    // CTAs of a row: enough to give every SM a few, as long as each of a CTA's warps has a group
-    const int step = 64 * static_cast<int>(16 / el);  // logits of one warp's loads
+    // CTAs of a row: as many as are resident at once (3 an SM), as long as each of a CTA's warps has a group
+    const int step = 128 * static_cast<int>(16 / el);  // logits of one warp's loads
     p.group = step;
     p.cluster = 1;
-    while (p.cluster < logprobs::MAX_CLUSTER && M * p.cluster < 4 * host::num_sms(dev) &&
-           V > static_cast<int64_t>(p.cluster) * 2 * logprobs::WARPS * step)
+    while (p.cluster < logprobs::MAX_CLUSTER && 2 * M * p.cluster <= 3 * host::num_sms(dev) &&
+           V > static_cast<int64_t>(p.cluster) * logprobs::WARPS * step)
         p.cluster *= 2;
-    const int limit = p.cluster > 1 ? 256 : logprobs::MAX_GROUPS;
+    const int limit = (p.cluster > 1 ? 256 : logprobs::MAX_GROUPS) / 2;  // two maxima a group
     auto groups = [&] { return (V + 16 + static_cast<int64_t>(p.group) * p.cluster - 1) / (static_cast<int64_t>(p.group) * p.cluster); };
     while (groups() > limit) p.group *= 2;
     p.groups = static_cast<int>(groups());
-    p.fine = p.cluster == 1 && p.group == step && p.groups * 64 <= logprobs::MAX_GROUPS;
+    p.fine = p.cluster == 1 && p.group == step && p.groups * 128 <= logprobs::MAX_GROUPS;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute pdl[1], attr[2];
     if (M * p.cluster > INT32_MAX) return LSE_ERR_UNSUPPORTED;

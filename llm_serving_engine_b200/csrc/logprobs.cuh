@@ -9,9 +9,10 @@
 //
 // One pass over the row, bound by DRAM where there are many rows and by latency where there are
 // few:
-//   * a warp reads a group of GROUP consecutive logits with 16-byte loads, takes its maximum,
-//     moves its running maximum m if it has to, and adds exp(x - m) and (x - m) exp(x - m) to its lanes'
-//     fp32 sums; with few rows a cluster of up to 8 CTAs shares one, joined through
+//   * a warp reads a group of consecutive logits with four 16-byte loads a lane (the next group's on
+//     their way), takes its maximum, moves its running maximum m if it has to, and adds 2^t and t 2^t,
+//     t = log2(e) x - r with r = log2(e) m as rounded, to its lanes' fp32 sums (any r will do as
+//     long as all use it: one FMA a logit); with few rows a cluster of up to 8 CTAs shares one, joined through
 //     distributed shared memory;
 //   * the alternatives come out of the groups' maxima: ordered by (maximum, index), the first k
 //     groups hold the k largest logits (of k other groups, each has an element that comes before
@@ -30,7 +31,7 @@ namespace logprobs {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 8;
-constexpr int MAX_GROUPS = 1024;   // groups of a CTA
+constexpr int MAX_GROUPS = 1024;   // maxima that a CTA keeps
 constexpr int MAX_TOP = LSE_LOGPROBS_MAX_TOP;
 constexpr int CANDIDATES = 512;    // logits ranked directly; more go round by round
 
@@ -43,7 +44,7 @@ struct Params {
     int64_t *top_id;        // [M, k]
     int M, V, k;
     int cluster;  // CTAs of a row
-    int group;    // logits of a group (a multiple of a warp's load of 32 x 16 bytes, x 2)
+    int group;    // logits of a group (a multiple of a warp's four loads of 32 x 16 bytes)
     int groups;   // groups of a CTA (rounded up)
     int fine;     // the alternatives come from the maxima of single 16-byte loads (short rows)
 };
@@ -67,6 +68,11 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error 2^-22; 2
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// Orders of -1e38 and 1e38: what lies outside overflows when scaled (rows of a type's lowest value, as a
+// mask leaves them, among it).
+constexpr unsigned ORDER_LOW = 0x01698966u, ORDER_HIGH = 0xfe967699u;
 
 // 16 bytes of logits as floats.
 template <typename T>
@@ -101,11 +107,13 @@ struct Vec {
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
-    constexpr int N = Vec<T>::N, STEP = 64 * N;  // logits of a warp's two loads
+    constexpr int N = Vec<T>::N, U = 4, STEP = 32 * U * N;  // logits of a warp's loads
+    constexpr int SUB = N == 8 ? 2 : 1;
     __shared__ unsigned s_top[MAX_GROUPS];       // order of each group's maximum
     __shared__ unsigned s_all[MAX_CLUSTER * 256];  // the row's (rank 0; fewer groups a CTA when it shares a row)
-    __shared__ float s_sum[WARPS][3];            // m, sum of exp, sum of (x - m) exp
+    __shared__ float s_sum[WARPS][3];            // m, sum of 2^t, sum of t 2^t
     __shared__ float s_row[3];                   // this CTA's
+    __shared__ unsigned s_lo;
     __shared__ int s_count, s_sel_n, s_sel[MAX_TOP];
     __shared__ unsigned long long s_key[CANDIDATES];
     __shared__ unsigned long long s_best[WARPS];
@@ -141,54 +149,88 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     };
 
     // ---- the pass: warp w takes groups w, w + WARPS, ... of this CTA -----------------------------------
+    // z = sum of 2^t, w = sum of t 2^t
+    auto between = [](float m0, float m1) { return __fmul_rn(m0, LOG2E) - __fmul_rn(m1, LOG2E); };
     float m = -INFINITY, z = 0.f, w = 0.f;
-    constexpr float LOG2E = 1.4426950408889634f;
     const int steps = p.group / STEP;  // of a group
-    auto group_at = [&](int g) { return cta0 + static_cast<int64_t>(g) * p.group + lane * N; };
+    const int sub = steps == 1 ? SUB : 1;  // the alternatives' groups in one of these
     auto live = [&](int g) { return g < p.groups && cta0 + static_cast<int64_t>(g) * p.group < end; };
-    Vec<T> a, b;
-    if (live(warp)) {
-        a = load(group_at(warp));
-        b = load(group_at(warp) + 32 * N);
-    }
+    auto load4 = [&](Vec<T> (&v)[U], int g, int i) {
+        const int64_t at = cta0 + static_cast<int64_t>(g) * p.group + i * STEP;
+        if (at >= shift && at + STEP <= end) {  // wholly inside the row
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(v[u].raw.x), "=r"(v[u].raw.y), "=r"(v[u].raw.z), "=r"(v[u].raw.w) : "l"(x0 + at + (32 * u + lane) * N));
+        } else {
+#pragma unroll 1
+            for (int u = 0; u < U; ++u) {
+                const Vec<T> one = load(at + (32 * u + lane) * N);
+                if (u == 0) v[0] = one;
+                else if (u == 1) v[1] = one;
+                else if (u == 2) v[2] = one;
+                else v[3] = one;
+            }
+        }
+    };
+    Vec<T> next[U];
+    if (live(warp)) load4(next, warp, 0);
     for (int g = warp; g < p.groups; g += WARPS) {
         unsigned best = 0;
         if (live(g))
             for (int i = 0; i < steps; ++i) {
-                const Vec<T> va = a, vb = b;
-                {  // the next loads
-                    const bool same = i + 1 < steps;
-                    const int ng = same ? g : g + WARPS;
-                    if (live(ng)) {
-                        const int64_t at = group_at(ng) + (same ? (i + 1) * STEP : 0);
-                        a = load(at);
-                        b = load(at + 32 * N);
-                    }
-                }
-                const unsigned ta = order_of(va.top()), tb = order_of(vb.top());
-                if (p.fine) {
-                    s_top[g * 64 + lane] = ta;
-                    s_top[g * 64 + 32 + lane] = tb;
-                }
-                const unsigned top = __reduce_max_sync(0xffffffffu, max(ta, tb));
-                best = max(best, top);
-                if (top <= ORDER_NONE || top >= ORDER_INF) continue;  // nothing to add; NaN and +inf show in the maximum
-                const float t = value_of(top);
-                if (t > m) {
-                    const float d = m - t, f = ex2(d * LOG2E);  // m = -inf: f = 0 and nothing was added
-                    w = z > 0.f ? f * fmaf(d, z, w) : 0.f;
-                    z *= f;
-                    m = t;
-                }
+                Vec<T> v[U];
 #pragma unroll
-                for (int k = 0; k < 2 * N; ++k) {
-                    const float d = fmaxf((k < N ? va[k] : vb[k - N]) - m, -1e30f);  // -inf: exp is 0, and 0 times it
-                    const float e = ex2(d * LOG2E);
-                    z += e;
-                    w = fmaf(d, e, w);
+                for (int u = 0; u < U; ++u) v[u] = next[u];
+                const bool same = i + 1 < steps;
+                if (live(same ? g : g + WARPS)) load4(next, same ? g : g + WARPS, same ? i + 1 : 0);
+                unsigned o[U], top = 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    o[u] = order_of(v[u].top());
+                    top = max(top, o[u]);
                 }
+                if (p.fine)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) s_top[g * (32 * U) + 32 * u + lane] = o[u];
+                // the alternatives' groups: SUB parts of a step
+                if constexpr (SUB == 2) {
+                    const unsigned t0 = __reduce_max_sync(0xffffffffu, max(o[0], o[1])), t1 = __reduce_max_sync(0xffffffffu, max(o[2], o[3]));
+                    top = max(t0, t1);
+                    if (steps == 1 && lane == 0 && !p.fine) {
+                        s_top[2 * g] = t0;
+                        s_top[2 * g + 1] = t1;
+                    }
+                } else {
+                    top = __reduce_max_sync(0xffffffffu, top);
+                }
+                best = max(best, top);
+                // nothing that counts beside an ordinary maximum; without one the row is done over below
+                if (top <= ORDER_LOW || top >= ORDER_HIGH) continue;
+                const float to = value_of(top);
+                if (to > m) {
+                    if (z > 0.f) {  // (m = -inf: nothing was added)
+                        const float d = between(m, to), f = ex2(d);
+                        w = f * fmaf(d, z, w);
+                        z *= f;
+                    }
+                    m = to;
+                }
+                const float r = __fmul_rn(m, LOG2E);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const float t = fmaxf(fmaf(v[u][k], LOG2E, -r), -1e30f);  // -inf: 2^t is 0, and t times it
+                        const float e = ex2(t);
+                        z += e;
+                        w = fmaf(t, e, w);
+                    }
             }
-        if (lane == 0 && !p.fine) s_top[g] = best;
+        if (lane == 0 && !p.fine) {
+            if (sub == 1) s_top[g] = best;
+            else if (!live(g)) s_top[2 * g] = s_top[2 * g + 1] = 0;
+        }
     }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) {
@@ -205,8 +247,8 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     auto join = [&](float &m0, float &z0, float &w0, float m1, float z1, float w1) {
         const float t = fmaxf(m0, m1);
         if (t == -INFINITY) return;
-        const float d0 = fmaxf(m0 - t, -1e30f), d1 = fmaxf(m1 - t, -1e30f);
-        const float f0 = ex2(d0 * LOG2E), f1 = ex2(d1 * LOG2E);
+        const float d0 = fmaxf(between(m0, t), -1e30f), d1 = fmaxf(between(m1, t), -1e30f);
+        const float f0 = ex2(d0), f1 = ex2(d1);
         w0 = f0 * fmaf(d0, z0, w0) + f1 * fmaf(d1, z1, w1);
         z0 = z0 * f0 + z1 * f1;
         m0 = t;
@@ -220,13 +262,13 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     }
     // ---- rank 0 has the row's sums and groups ---------------------------------------------------------
     const unsigned *tops = s_top;
-    const int all = p.fine ? min(p.groups * 64, static_cast<int>((end + N - 1) / N)) : p.groups * p.cluster;
-    const int group = p.fine ? N : p.group;
+    const int all = p.fine ? min(p.groups * 32 * U, static_cast<int>((end + N - 1) / N)) : p.groups * sub * p.cluster;
+    const int group = p.fine ? N : p.group / sub, mine_n = p.groups * sub;
     if (p.cluster > 1) {
         ptx::cluster_sync();
         if (rank == 0) {
             for (int i = threadIdx.x; i < all; i += THREADS) {
-                const uint32_t at = ptx::map_shared_rank(ptx::smem_u32(&s_top[i % p.groups]), i / p.groups);
+                const uint32_t at = ptx::map_shared_rank(ptx::smem_u32(&s_top[i % mine_n]), i / mine_n);
                 asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(s_all[i]) : "r"(at) : "memory");
             }
             if (threadIdx.x == 0)
@@ -252,12 +294,47 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     unsigned most = 0;
     for (int i = threadIdx.x; i < all; i += THREADS) most = max(most, tops[i]);
     const bool nan = __syncthreads_or(most >= ORDER_INF);
-    const float top = s_row[0], zz = s_row[1], ww = s_row[2];
-    const bool empty = top == -INFINITY && !nan;
-    const float log_z = logf(zz), none = __int_as_float(0x7fffffff);
-    auto lp = [&](float v) { return nan ? none : empty ? -INFINITY : (v - top) - log_z; };
+    unsigned largest = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) s_best[warp] = largest;
+    __syncthreads();
+    for (int i = 0; i < WARPS; ++i) largest = max(largest, static_cast<unsigned>(s_best[i]));
+    const bool empty = largest <= ORDER_NONE, huge = !nan && !empty && (largest <= ORDER_LOW || largest >= ORDER_HIGH);
+    if (huge) {  // differences first, then the scale: an element at a time, by this CTA alone
+        const float top = value_of(largest);
+        float z1 = 0.f, w1 = 0.f;
+        for (int i = threadIdx.x; i < p.V; i += THREADS) {
+            const float d = fmaxf(to_float(x[i]) - top, -1e30f) * LOG2E, e = ex2(d);
+            z1 += e;
+            w1 = fmaf(d, e, w1);
+        }
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) {
+            z1 += __shfl_xor_sync(0xffffffffu, z1, k);
+            w1 += __shfl_xor_sync(0xffffffffu, w1, k);
+        }
+        if (lane == 0) {
+            s_sum[warp][1] = z1;
+            s_sum[warp][2] = w1;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            s_row[0] = top;
+            s_row[1] = s_row[2] = 0.f;
+            for (int i = 0; i < WARPS; ++i) {
+                s_row[1] += s_sum[i][1];
+                s_row[2] += s_sum[i][2];
+            }
+        }
+        __syncthreads();
+    }
+    const float ref = s_row[0], log_z = log2f(s_row[1]), none = __int_as_float(0x7fffffff);
+    auto lp = [&](float v) {
+        if (nan || empty) return nan ? none : -INFINITY;
+        if (huge || fabsf(v) > 1e38f) return (v - ref) - log_z * LN2;
+        return (fmaf(v, LOG2E, -__fmul_rn(ref, LOG2E)) - log_z) * LN2;
+    };
     if (threadIdx.x == 0) {
-        p.entropy[row] = nan ? none : empty ? 0.f : log_z - ww / zz;
+        p.entropy[row] = nan ? none : empty ? 0.f : (log_z - s_row[2] / s_row[1]) * LN2;
         if (p.tokens) {
             const int64_t t = p.tokens[row];
             const bool in = t >= 0 && t < p.V;
@@ -269,52 +346,73 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 
     // ---- the first k groups by (maximum, index) -------------------------------------------------------
     const int want = min(p.k, all);
-    // a T that `want` groups reach (and so k logits), the largest or one with no group's maximum between;
-    // 0 where there are no k groups
-    unsigned lo = 0, hi = want < p.k ? 0u : 0xffffffffu;  // count(>= lo) >= want
-    int reach = all;
-    while (lo < hi) {
-        const unsigned mid = lo + (hi - lo) / 2 + 1;
-        int n = 0;
-        for (int i0 = 0; i0 < all; i0 += THREADS) n += __syncthreads_count(i0 + threadIdx.x < all && tops[i0 + threadIdx.x] >= mid);
-        if (n >= want) {
-            lo = mid;
-            reach = n;
-            if (n == want) break;  // any threshold between gives the same groups
-        } else {
-            hi = mid - 1;
+    // `lo`: an order that `want` groups reach (and so k logits) and, among equal ones aside, no other; 0 where
+    // there are no k groups.
+    unsigned lo = 0;
+    if (all <= THREADS) {  // every group counts those before it
+        const int i = threadIdx.x;
+        if (i < all) {
+            const unsigned mine = tops[i];
+            int before = 0;
+#pragma unroll 4
+            for (int j = 0; j < all; ++j) {
+                const unsigned o = tops[j];
+                before += o > mine || (o == mine && j < i);
+            }
+            if (before < want) s_sel[before] = i;
+            if (before == want - 1) s_lo = want < p.k ? 0u : mine;
         }
-    }
-    if (warp == 0) {  // those above T, then those at T from the lowest index on
-        int above = 0;
-        for (int i0 = 0; i0 < all; i0 += 32) above += __popc(__ballot_sync(0xffffffffu, i0 + lane < all && tops[i0 + lane] > lo));
-        int level = reach == want ? want : want - above;  // groups at T that still fit (all of them when the count is exact)
-        int n = 0;
-        for (int i0 = 0; i0 < all; i0 += 32) {
-            const unsigned o = i0 + lane < all ? tops[i0 + lane] : 0u;
-            const bool in = i0 + lane < all && o >= lo, at = in && o == lo;
-            const unsigned eq = __ballot_sync(0xffffffffu, at);
-            const bool take = in && (!at || __popc(eq & ((1u << lane) - 1u)) < level);
-            const unsigned yes = __ballot_sync(0xffffffffu, take);
-            if (take) s_sel[n + __popc(yes & ((1u << lane) - 1u))] = i0 + lane;
-            n += __popc(yes);
-            level -= __popc(eq & yes);
+        if (i == 0) s_sel_n = want;
+        __syncthreads();
+        lo = s_lo;
+    } else {
+        unsigned hi = want < p.k ? 0u : 0xffffffffu;  // count(>= lo) >= want
+        int reach = all;
+        while (lo < hi) {
+            const unsigned mid = lo + (hi - lo) / 2 + 1;
+            int n = 0;
+            for (int i0 = 0; i0 < all; i0 += THREADS) n += __syncthreads_count(i0 + threadIdx.x < all && tops[i0 + threadIdx.x] >= mid);
+            if (n >= want) {
+                lo = mid;
+                reach = n;
+                if (n == want) break;  // any threshold between gives the same groups
+            } else {
+                hi = mid - 1;
+            }
         }
-        if (lane == 0) s_sel_n = n;
+        if (warp == 0) {  // those above, then those at `lo` from the lowest index on
+            int above = 0;
+            for (int i0 = 0; i0 < all; i0 += 32) above += __popc(__ballot_sync(0xffffffffu, i0 + lane < all && tops[i0 + lane] > lo));
+            int level = reach == want ? want : want - above;  // groups at `lo` that still fit (all of them when the count is exact)
+            int n = 0;
+            for (int i0 = 0; i0 < all; i0 += 32) {
+                const unsigned o = i0 + lane < all ? tops[i0 + lane] : 0u;
+                const bool in = i0 + lane < all && o >= lo, at = in && o == lo;
+                const unsigned eq = __ballot_sync(0xffffffffu, at);
+                const bool take = in && (!at || __popc(eq & ((1u << lane) - 1u)) < level);
+                const unsigned yes = __ballot_sync(0xffffffffu, take);
+                if (take) s_sel[n + __popc(yes & ((1u << lane) - 1u))] = i0 + lane;
+                n += __popc(yes);
+                level -= __popc(eq & yes);
+            }
+            if (lane == 0) s_sel_n = n;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const int sel_n = s_sel_n;
-    // Keys of the logits of the selected groups: a warp's 16 bytes a lane at a time, or a lane's own (fine).
+    // Keys of the logits of the selected groups, a thread 16 bytes at a time.
+    const int vecs = group / N;  // of a group
     auto visit = [&](auto f) {
-        for (int s = p.fine ? threadIdx.x : warp; s < sel_n; s += p.fine ? THREADS : WARPS) {
-            const int64_t g0 = static_cast<int64_t>(s_sel[s]) * group;  // (ranks' groups follow one another)
-            for (int64_t at = g0 + (p.fine ? 0 : lane * N); at < min(g0 + group, end); at += 32 * N) {
-                const Vec<T> v = load(at);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < sel_n * vecs; i += THREADS) {
+            const int64_t at = static_cast<int64_t>(s_sel[i / vecs]) * group + (i % vecs) * N;  // (ranks' groups follow one another)
+            if (at >= end) continue;
+            const Vec<T> v = load(at);
+            if (order_of(v.top()) < lo) continue;
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const int64_t i = at + k - shift;
-                    if (i >= 0 && i < p.V) f((static_cast<unsigned long long>(order_of(v[k])) << 32) | (0x7fffffffu - static_cast<unsigned>(i)));
-                }
+            for (int k = 0; k < N; ++k) {
+                const int64_t e = at + k - shift;
+                if (e >= 0 && e < p.V) f((static_cast<unsigned long long>(order_of(v[k])) << 32) | (0x7fffffffu - static_cast<unsigned>(e)));
             }
         }
     };
