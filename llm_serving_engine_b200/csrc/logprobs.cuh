@@ -33,6 +33,7 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_GROUPS = 1024;   // maxima that a CTA keeps
 constexpr int MAX_TOP = LSE_LOGPROBS_MAX_TOP;
+constexpr int ROUNDS = 32;         // alternatives whose groups one warp picks in turn
 constexpr int CANDIDATES = 512;    // logits ranked directly; more go round by round
 
 struct Params {
@@ -106,13 +107,13 @@ struct Vec {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, 3) rows_kernel(const Params p) {
     constexpr int N = Vec<T>::N, U = 4, STEP = 32 * U * N;  // logits of a warp's loads
     constexpr int SUB = N == 8 ? 2 : 1;
     __shared__ unsigned s_top[MAX_GROUPS];       // order of each group's maximum
     __shared__ unsigned s_all[MAX_CLUSTER * 256];  // the row's (rank 0; fewer groups a CTA when it shares a row)
-    __shared__ float s_sum[WARPS][3];            // m, sum of 2^t, sum of t 2^t
-    __shared__ float s_row[3];                   // this CTA's
+    __shared__ float s_sum[WARPS][4];            // m, sum of 2^t, sum of t 2^t, order of the maximum
+    __shared__ float s_row[4];                   // this CTA's
     __shared__ unsigned s_lo;
     __shared__ int s_count, s_sel_n, s_sel[MAX_TOP];
     __shared__ unsigned long long s_key[CANDIDATES];
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     // z = sum of 2^t, w = sum of t 2^t
     auto between = [](float m0, float m1) { return __fmul_rn(m0, LOG2E) - __fmul_rn(m1, LOG2E); };
     float m = -INFINITY, z = 0.f, w = 0.f;
+    unsigned largest = 0;  // order of the warp's maximum
     const int steps = p.group / STEP;  // of a group
     const int sub = steps == 1 ? SUB : 1;  // the alternatives' groups in one of these
     auto live = [&](int g) { return g < p.groups && cta0 + static_cast<int64_t>(g) * p.group < end; };
@@ -227,6 +229,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
                         w = fmaf(t, e, w);
                     }
             }
+        largest = max(largest, best);
         if (lane == 0 && !p.fine) {
             if (sub == 1) s_top[g] = best;
             else if (!live(g)) s_top[2 * g] = s_top[2 * g + 1] = 0;
@@ -241,24 +244,37 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
         s_sum[warp][0] = m;
         s_sum[warp][1] = z;
         s_sum[warp][2] = w;
+        s_sum[warp][3] = __uint_as_float(largest);
     }
     __syncthreads();
-    // Joins (m, z, w) triples; the order is fixed.
-    auto join = [&](float &m0, float &z0, float &w0, float m1, float z1, float w1) {
-        const float t = fmaxf(m0, m1);
-        if (t == -INFINITY) return;
-        const float d0 = fmaxf(between(m0, t), -1e30f), d1 = fmaxf(between(m1, t), -1e30f);
-        const float f0 = ex2(d0), f1 = ex2(d1);
-        w0 = f0 * fmaf(d0, z0, w0) + f1 * fmaf(d1, z1, w1);
-        z0 = z0 * f0 + z1 * f1;
-        m0 = t;
+    // Joins eight (m, z, w, largest), one in each of lanes 0-7, into all of them; the order is fixed.
+    static_assert(WARPS == 8 && MAX_CLUSTER == 8, "one per lane");
+    auto join = [&] {
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) {
+            const float m1 = __shfl_xor_sync(0xffffffffu, m, k), z1 = __shfl_xor_sync(0xffffffffu, z, k), w1 = __shfl_xor_sync(0xffffffffu, w, k);
+            const float t = fmaxf(m, m1);
+            const float d0 = t == -INFINITY ? 0.f : fmaxf(between(m, t), -1e30f), d1 = t == -INFINITY ? 0.f : fmaxf(between(m1, t), -1e30f);
+            const float f0 = ex2(d0), f1 = ex2(d1), a0 = f0 * fmaf(d0, z, w), a1 = f1 * fmaf(d1, z1, w1);
+            w = lane & k ? a1 + a0 : a0 + a1;
+            z = lane & k ? z1 * f1 + z * f0 : z * f0 + z1 * f1;
+            m = t;
+            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, k));
+        }
     };
-    if (threadIdx.x == 0) {
-        float m0 = -INFINITY, z0 = 0.f, w0 = 0.f;
-        for (int i = 0; i < WARPS; ++i) join(m0, z0, w0, s_sum[i][0], s_sum[i][1], s_sum[i][2]);
-        s_row[0] = m0;
-        s_row[1] = z0;
-        s_row[2] = w0;
+    if (warp == 0) {
+        m = lane < WARPS ? s_sum[lane][0] : -INFINITY;
+        z = lane < WARPS ? s_sum[lane][1] : 0.f;
+        w = lane < WARPS ? s_sum[lane][2] : 0.f;
+        largest = lane < WARPS ? __float_as_uint(s_sum[lane][3]) : 0u;
+        join();
+        if (lane == 0) {
+            s_row[0] = m;
+            s_row[1] = z;
+            s_row[2] = w;
+            s_row[3] = __uint_as_float(largest);
+            s_count = 0;
+        }
     }
     // ---- rank 0 has the row's sums and groups ---------------------------------------------------------
     const unsigned *tops = s_top;
@@ -267,54 +283,57 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     if (p.cluster > 1) {
         ptx::cluster_sync();
         if (rank == 0) {
-            for (int i = threadIdx.x; i < all; i += THREADS) {
-                const uint32_t at = ptx::map_shared_rank(ptx::smem_u32(&s_top[i % mine_n]), i / mine_n);
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(s_all[i]) : "r"(at) : "memory");
-            }
-            if (threadIdx.x == 0)
-                for (int r = 1; r < p.cluster; ++r) {
-                    float v[3];
+            if (p.k)
+                for (int i = threadIdx.x; i < all; i += THREADS) {
+                    const uint32_t at = ptx::map_shared_rank(ptx::smem_u32(&s_top[i % mine_n]), i / mine_n);
+                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(s_all[i]) : "r"(at) : "memory");
+                }
+            if (warp == 0) {
+                float v[4] = {-INFINITY, 0.f, 0.f, 0.f};
+                if (lane < p.cluster)
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) {
-                        const uint32_t at = ptx::map_shared_rank(ptx::smem_u32(&s_row[i]), r);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t at = ptx::map_shared_rank(ptx::smem_u32(&s_row[i]), lane);
                         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i]) : "r"(at) : "memory");
                     }
-                    join(s_row[0], s_row[1], s_row[2], v[0], v[1], v[2]);
+                m = v[0];
+                z = v[1];
+                w = v[2];
+                largest = __float_as_uint(v[3]);
+                join();
+                if (lane == 0) {
+                    s_row[0] = m;
+                    s_row[1] = z;
+                    s_row[2] = w;
+                    s_row[3] = __uint_as_float(largest);
                 }
+            }
             tops = s_all;
         }
         ptx::cluster_sync();  // the other CTAs' shared memory has been read
         if (rank != 0) return;
+    } else {
+        __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        s_count = 0;
-        s_sel_n = 0;
-    }
-    __syncthreads();
-    unsigned most = 0;
-    for (int i = threadIdx.x; i < all; i += THREADS) most = max(most, tops[i]);
-    const bool nan = __syncthreads_or(most >= ORDER_INF);
-    unsigned largest = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) s_best[warp] = largest;
-    __syncthreads();
-    for (int i = 0; i < WARPS; ++i) largest = max(largest, static_cast<unsigned>(s_best[i]));
+    largest = __float_as_uint(s_row[3]);
+    const bool nan = largest >= ORDER_INF;
     const bool empty = largest <= ORDER_NONE, huge = !nan && !empty && (largest <= ORDER_LOW || largest >= ORDER_HIGH);
     if (huge) {  // differences first, then the scale: an element at a time, by this CTA alone
         const float top = value_of(largest);
-        float z1 = 0.f, w1 = 0.f;
+        z = w = 0.f;
         for (int i = threadIdx.x; i < p.V; i += THREADS) {
             const float d = fmaxf(to_float(x[i]) - top, -1e30f) * LOG2E, e = ex2(d);
-            z1 += e;
-            w1 = fmaf(d, e, w1);
+            z += e;
+            w = fmaf(d, e, w);
         }
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) {
-            z1 += __shfl_xor_sync(0xffffffffu, z1, k);
-            w1 += __shfl_xor_sync(0xffffffffu, w1, k);
+            z += __shfl_xor_sync(0xffffffffu, z, k);
+            w += __shfl_xor_sync(0xffffffffu, w, k);
         }
         if (lane == 0) {
-            s_sum[warp][1] = z1;
-            s_sum[warp][2] = w1;
+            s_sum[warp][1] = z;
+            s_sum[warp][2] = w;
         }
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -333,7 +352,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
         if (huge || fabsf(v) > 1e38f) return (v - ref) - log_z * LN2;
         return (fmaf(v, LOG2E, -__fmul_rn(ref, LOG2E)) - log_z) * LN2;
     };
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == THREADS - 1) {  // (not of the warp that selects below)
         p.entropy[row] = nan ? none : empty ? 0.f : (log_z - s_row[2] / s_row[1]) * LN2;
         if (p.tokens) {
             const int64_t t = p.tokens[row];
@@ -349,20 +368,39 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     // `lo`: an order that `want` groups reach (and so k logits) and, among equal ones aside, no other; 0 where
     // there are no k groups.
     unsigned lo = 0;
-    if (all <= THREADS) {  // every group counts those before it
-        const int i = threadIdx.x;
-        if (i < all) {
-            const unsigned mine = tops[i];
-            int before = 0;
-#pragma unroll 4
-            for (int j = 0; j < all; ++j) {
-                const unsigned o = tops[j];
-                before += o > mine || (o == mine && j < i);
+    if (p.k <= ROUNDS && all <= 32 * 32) {  // one warp, a group a round: lane l has groups l, l + 32, ... in registers
+        auto pick = [&](auto lanes_groups) {
+            constexpr int Q = decltype(lanes_groups)::value;
+            unsigned key[Q], top = 0;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) key[q] = lane + 32 * q < all ? tops[lane + 32 * q] : 0u;
+            int n = 0;
+            for (; n < want; ++n) {
+                unsigned mine = 0;
+                int at = 0x7fffffff;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (key[q] > mine) {
+                        mine = key[q];
+                        at = lane + 32 * q;
+                    }
+                top = __reduce_max_sync(0xffffffffu, mine);
+                if (top == 0) break;  // what is left holds nothing of the row
+                const int i = __reduce_min_sync(0xffffffffu, mine == top ? at : 0x7fffffff);
+                if (lane == 0) s_sel[n] = i;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (lane + 32 * q == i) key[q] = 0;  // taken
             }
-            if (before < want) s_sel[before] = i;
-            if (before == want - 1) s_lo = want < p.k ? 0u : mine;
+            if (lane == 0) {
+                s_lo = n < p.k ? 0u : top;
+                s_sel_n = n;
+            }
+        };
+        if (warp == 0) {
+            if (all <= 8 * 32) pick(std::integral_constant<int, 8>{});
+            else pick(std::integral_constant<int, 32>{});
         }
-        if (i == 0) s_sel_n = want;
         __syncthreads();
         lo = s_lo;
     } else {
