@@ -156,29 +156,41 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
 
     // ---- the run of chunks of this CTA -------------------------------------------------------
     // Every CTA adds up all lengths (E is small); an entry has chunks_of(context) * H_kv chunks.
-    int64_t total = 0;
-    int longest = 0;
-    for (int e0 = 0; e0 < p.E; e0 += DEC_THREADS) {
+    // A round is DEC_THREADS entries; `round` leaves this thread's entry's chunks and those before it.
+    int n_mine = 0, ctx_mine = 0, before = 0, longest = 0;
+    int64_t base = 0;  // chunks (of one KV head) of the rounds so far
+    auto round = [&](int e0, bool first) {
         const int e = e0 + threadIdx.x;
-        int n = 0;
+        n_mine = ctx_mine = 0;
         if (e < p.E) {
-            n = chunks_of(context(e));
-            if (blockIdx.x == 0 && __ldcg(p.context_len + e) > table_positions) report_status(LSE_ERR_INVALID_ARG);
+            const int c = __ldcg(p.context_len + e);
+            ctx_mine = static_cast<int>(min(static_cast<int64_t>(max(c, 0)), table_positions));
+            n_mine = chunks_of(ctx_mine);
+            if (first && blockIdx.x == 0 && c > table_positions) report_status(LSE_ERR_INVALID_ARG);
         }
-        const int sum = __reduce_add_sync(0xffffffffu, n), mx = __reduce_max_sync(0xffffffffu, n);
-        if (lane == 0) {
-            s_scan[warp] = sum;
+        int incl = n_mine;
+#pragma unroll
+        for (int k = 1; k < 32; k <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, k);
+            if (lane >= k) incl += v;
+        }
+        const int mx = __reduce_max_sync(0xffffffffu, n_mine);
+        if (lane == 31) {
+            s_scan[warp] = incl;
             s_max[warp] = mx;
         }
         __syncthreads();
+        before = incl - n_mine;
 #pragma unroll
         for (int i = 0; i < DEC_WARPS; ++i) {
-            total += s_scan[i];
+            if (i < warp) before += s_scan[i];
+            base += s_scan[i];
             longest = max(longest, s_max[i]);
         }
         __syncthreads();
-    }
-    total *= p.H_kv;
+    };
+    for (int e0 = 0; e0 < p.E; e0 += DEC_THREADS) round(e0, true);
+    const int64_t total = base * p.H_kv;
     // CTAs in use: no more than there are chunks, nor than leave a pair in DEC_MAX_SPLITS pieces
     const int64_t active = min(min(static_cast<int64_t>(gridDim.x), total), max(static_cast<int64_t>(1), DEC_MAX_SPLITS * total / longest));
     if (blockIdx.x >= active) return;
@@ -187,46 +199,26 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
     auto cta_of = [&](int64_t chunk) { return static_cast<int>(((chunk + 1) * active - 1) / total); };
 
     // the entry that chunk `at` belongs to, and the first chunk of that entry
-    int e = 0;
-    int64_t e_first = 0;
-    {
-        int64_t base = 0;
-        for (int e0 = 0; e0 < p.E; e0 += DEC_THREADS) {
-            const int i = e0 + threadIdx.x;
-            int n = i < p.E ? chunks_of(context(i)) : 0, incl = n;
-#pragma unroll
-            for (int k = 1; k < 32; k <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, k);
-                if (lane >= k) incl += v;
-            }
-            if (lane == 31) s_scan[warp] = incl;
-            if (threadIdx.x == 0) s_at[0] = -1;
-            __syncthreads();
-            int before = incl - n, all = 0;
-#pragma unroll
-            for (int k = 0; k < DEC_WARPS; ++k) {
-                if (k < warp) before += s_scan[k];
-                all += s_scan[k];
-            }
-            const int64_t first = (base + before) * p.H_kv, last = first + static_cast<int64_t>(n) * p.H_kv;
-            if (n > 0 && at >= first && at < last) {
-                s_at[0] = i;
-                s_at[1] = static_cast<int>(at - first);
-            }
-            __syncthreads();
-            const bool found = s_at[0] >= 0;
-            if (found) {
-                e = s_at[0];
-                e_first = at - s_at[1];
-                break;
-            }
-            base += all;
+    base = 0;
+    if (threadIdx.x == 0) s_at[0] = -1;
+    __syncthreads();
+    for (int e0 = 0; e0 < p.E; e0 += DEC_THREADS) {
+        const int64_t here = base;
+        if (p.E > DEC_THREADS) round(e0, false);  // (one round: its values are still here)
+        const int64_t first = (here + before) * p.H_kv;
+        if (n_mine > 0 && at >= first && at < first + static_cast<int64_t>(n_mine) * p.H_kv) {
+            s_at[0] = e0 + threadIdx.x;
+            s_at[1] = static_cast<int>(at - first);
+            s_at[2] = ctx_mine;
         }
         __syncthreads();
+        if (s_at[0] >= 0) break;
     }
+    int e = s_at[0], ctx = s_at[2];
+    int64_t e_first = at - s_at[1];
+    __syncthreads();  // s_at[2] is used again
 
     while (at < end) {
-        const int ctx = context(e);
         const int n = chunks_of(ctx);
         const int kvh = static_cast<int>((at - e_first) / n);
         const int64_t pair_first = e_first + static_cast<int64_t>(kvh) * n, pair_end = pair_first + n;
@@ -236,11 +228,10 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
         const int pos1 = min(ctx, static_cast<int>(stop - pair_first) * CHUNK);
 
         // ---- q: the column operand (heads as columns), k-step j of chunk q4 + 4c: dims 16 (q4 + 4c) + 4 (j % 4) ..
-        uint32_t qb[4 * KC][2];
-        float back = 1.f;  // what q's scaling took off
+        uint32_t qb[4 * KC][2], raw[8 * KC];
+        float c0, c1;  // score factors of this thread's columns of S^T: heads 2 q4 and 2 q4 + 1
         {
             const T *qp = static_cast<const T *>(p.q) + e * p.q_st + static_cast<int64_t>(kvh * G + r0) * p.q_sh;
-            uint32_t raw[8 * KC];
 #pragma unroll
             for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -252,6 +243,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
                     raw[8 * c + 4 * i + 2] = v.z;
                     raw[8 * c + 4 * i + 3] = v.w;
                 }
+        }
+        auto load_q = [&] {
+            float back = 1.f;  // what q's scaling takes off
             if constexpr (std::is_same_v<T, __half>) {
 #pragma unroll
                 for (int i = 0; i < 8 * KC; ++i) qb[i / 2][i % 2] = raw[i];
@@ -275,10 +269,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
                     qb[i / 2][i % 2] = half2_of(f.x * down, f.y * down);
                 }
             }
-        }
-        // this thread's columns of S^T: heads 2 q4 and 2 q4 + 1
-        const float c0 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * q4);
-        const float c1 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * q4 + 4);
+            c0 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * q4);
+            c1 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * q4 + 4);
+        };
 
         float m0 = M_NONE, m1 = M_NONE, l0 = 0.f, l1 = 0.f;
         float acc[MT][4];
@@ -310,7 +303,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
         // Here lane 2 U i + g works for group g (8 positions) of tile i of the window.
         auto group_pos = [&](int window) { return tile_pos(window * WIN + lane / (2 * U)) + 8 * (lane % (2 * U)); };
         auto lookup = [&](int window) { return window * WIN + lane / (2 * U) < mine ? page_of(group_pos(window)) : -1; };
-        int blk_pending = -1, blk_scaled = -1;
+        int blk_pending = PAGED8 ? lookup(0) : -1, blk_scaled = -1;
         float k_pending = 0.f, v_pending = 0.f;
         unsigned dead_windows = 0;  // bit (window & 1): it holds pages that are not to be read
         auto load_scales = [&](int window) {  // of the window whose block ids are pending, and the next one's ids
@@ -318,9 +311,14 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
             scales(blk_scaled, k_pending, v_pending);
             blk_pending = lookup(window + 1);
         };
-        auto write_table = [&](int window) {
+        auto write_row = [&](int window) {  // the group's first row, which the copies need
             const int per = p.block_size >> 3;
             const int row8 = blk_scaled < 0 ? -1 : (blk_scaled * p.H_kv + kvh) * per + (group_pos(window) >> 3) % per;
+            s_table[warp][window & 1][lane].x = __int_as_float(row8);
+            return row8;
+        };
+        auto write_table = [&](int window) {
+            const int row8 = write_row(window);
             s_table[warp][window & 1][lane] = make_float4(__int_as_float(row8), k_pending, v_pending, fmaxf(fabsf(v_pending), V_LEAST));
             const bool gone = row8 < 0 && window * WIN + lane / (2 * U) < mine && group_pos(window) < pos1;
             const unsigned bit = 1u << (window & 1);
@@ -367,12 +365,16 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
         };
 
         if constexpr (PAGED8) {
-            blk_pending = lookup(0);
             load_scales(0);
+            write_row(0);
+            __syncwarp();
+        }
+        for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
+        load_q();  // (its loads went out before the look-ups)
+        if constexpr (PAGED8) {  // the scales come in while the first tiles do
             write_table(0);
             load_scales(1);
         }
-        for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
         int slot = 0;
         for (int i = 0; i < mine; ++i) {
             if constexpr (PAGED8) {
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
         at = stop;
         if (at == e_first + static_cast<int64_t>(n) * p.H_kv) {
             e_first = at;
-            ++e;
+            if (++e < p.E) ctx = context(e);
         }
     }
 }
