@@ -584,16 +584,34 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
             if (s_at[2]) {
                 __threadfence();
                 auto slot_of = [&](int i) { return static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)); };
+                // eight pieces' sums at a time, the first eight on their way under the weights
+                constexpr int BATCH = 8;
+                float4 v[BATCH];
+                auto fetch = [&](int i, int k0) {
+#pragma unroll
+                    for (int u = 0; u < BATCH; ++u)
+                        if (k0 + u < pieces) v[u] = __ldcg(reinterpret_cast<const float4 *>(w.acc + slot_of(k0 + u) * (G * D) + i));
+                };
+                if (4 * threadIdx.x < G * D) fetch(4 * threadIdx.x, 0);
                 for (int h = warp; h < G; h += DEC_WARPS) {
-                    float M = M_NONE;
-                    for (int i = lane; i < pieces; i += 32) M = fmaxf(M, __ldcg(w.ml + (slot_of(i) * G + h) * 2));
+                    float M = M_NONE, m[(DEC_MAX_SPLITS + 33) / 32], l[(DEC_MAX_SPLITS + 33) / 32];
+#pragma unroll
+                    for (int x = 0; x < (DEC_MAX_SPLITS + 33) / 32; ++x) {
+                        const int i = lane + 32 * x;
+                        const float2 ml = i < pieces ? __ldcg(reinterpret_cast<const float2 *>(w.ml) + slot_of(i) * G + h) : make_float2(M_NONE, 0.f);
+                        m[x] = ml.x;
+                        l[x] = ml.y;
+                        M = fmaxf(M, ml.x);
+                    }
 #pragma unroll
                     for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
                     float L = 0.f;
-                    for (int i = lane; i < pieces; i += 32) {
-                        const float f = ex2_approx(__ldcg(w.ml + (slot_of(i) * G + h) * 2) - M);
-                        s_w[i][h] = f;
-                        L += f * __ldcg(w.ml + (slot_of(i) * G + h) * 2 + 1);
+#pragma unroll
+                    for (int x = 0; x < (DEC_MAX_SPLITS + 33) / 32; ++x) {
+                        const int i = lane + 32 * x;
+                        const float f = ex2_approx(m[x] - M);
+                        if (i < pieces) s_w[i][h] = f;
+                        L += f * l[x];
                     }
 #pragma unroll
                     for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
@@ -603,14 +621,17 @@ __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams
                 for (int i = 4 * threadIdx.x; i < G * D; i += 4 * DEC_THREADS) {
                     const int h = i / D;
                     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int k = 0; k < pieces; ++k) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(w.acc + slot_of(k) * (G * D) + i));
-                        const float f = s_w[k][h];
-                        A.x = fmaf(v.x, f, A.x);
-                        A.y = fmaf(v.y, f, A.y);
-                        A.z = fmaf(v.z, f, A.z);
-                        A.w = fmaf(v.w, f, A.w);
+                    for (int k0 = 0; k0 < pieces; k0 += BATCH) {
+                        if (k0 > 0 || i >= 4 * DEC_THREADS) fetch(i, k0);
+#pragma unroll
+                        for (int u = 0; u < BATCH; ++u)
+                            if (k0 + u < pieces) {
+                                const float f = s_w[k0 + u][h];
+                                A.x = fmaf(v[u].x, f, A.x);
+                                A.y = fmaf(v[u].y, f, A.y);
+                                A.z = fmaf(v[u].z, f, A.z);
+                                A.w = fmaf(v[u].w, f, A.w);
+                            }
                     }
                     const float L = s_l[h], inv = L != 0.f ? 1.f / L : 0.f;
                     T *dst = o + h * p.o_sh + i % D;
