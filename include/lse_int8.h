@@ -332,9 +332,9 @@ const char *lse_last_cuda_error(void);
 /*
  * Device-side status of `device`: LSE_OK, or LSE_ERR_DEVICE_TIMEOUT when a bounded
  * wait inside a kernel gave up since the last reset.  Synchronizes the device.  When
- * `reset` is nonzero the flag is cleared.  After a timeout the decode-attention workspace
- * (lse_paged_decode_attention) must be zeroed again before its next use; the linear
- * workspaces need nothing.
+ * `reset` is nonzero the flag is cleared.  After a timeout the attention workspaces
+ * (lse_paged_decode_attention, lse_kv8_decode_attention, lse_kv8_paged_attention) must be zeroed
+ * again before their next use; the linear workspaces need nothing.
  */
 int lse_device_status(int device, int reset);
 

@@ -119,7 +119,7 @@ struct PromptSchedule {
         } else {
             while (at >= first + nq * p.H_kv) {
                 first += nq * p.H_kv;
-                ++e;
+                if (++e >= p.E) return false;
                 load_entry(p);
             }
             const int k = at - first;
@@ -235,6 +235,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
         ptx::fence_mbar_init();
         s_abort_word = 0;
     }
+    // (after a wait that ran out the loads go by rows that may not have been written yet: any row of the pool)
+    for (int i = threadIdx.x; i < 2 * PR_KEYS; i += PR_THREADS) s_rows[i / PR_KEYS][i % PR_KEYS] = 0;
     if (warp == PR_MMA) {
         ptx::tmem_alloc(ptx::smem_u32(&s_tmem), 512);
         ptx::tmem_relinquish();
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
                     uint32_t pk[16];
                     float add[2];
                     ptx::tmem_wait_ld();
-                    while (true) {
+                    for (int again = 0;; ++again) {  // at most once more, with M moved
                         bool over;  // a weight is over 2^6 as it would meet V
                         add[0] = add[1] = 0.f;
                         if (!masks) {
@@ -476,7 +478,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
                                 pk[k] = half2_of(y[0], y[1]);
                             }
                         }
-                        if (!__any_sync(0xffffffffu, over)) break;
+                        // (scales that overflow, or what a wait that ran out left behind, may be over for good)
+                        if (again || !__any_sync(0xffffffffu, over)) break;
                         // M moves for some row of the warp
                         float top = M;
 #pragma unroll

@@ -188,24 +188,33 @@ at::Tensor rows16(const at::Tensor &x) {
 // kernel, kept between calls and grown (never inside a capture) when a call needs more.  A
 // stream capture has a buffer of its own, allocated and zeroed by the captured work, so that a
 // replay shares nothing with eager calls on any stream.
+using WorkspaceKey = std::tuple<int, int, cudaStream_t>;
+std::mutex g_workspace_lock;
+auto &g_workspaces = *new std::map<WorkspaceKey, at::Tensor>();  // alive to the process's end
+auto &g_captured_workspaces = *new std::map<WorkspaceKey, std::pair<unsigned long long, at::Tensor>>();
+
 at::Tensor counters_workspace(int which, size_t bytes, const at::Tensor &like, cudaStream_t stream) {
-    static std::mutex lock;
-    static auto &kept = *new std::map<std::tuple<int, int, cudaStream_t>, at::Tensor>();  // alive to the process's end
-    static auto &captured = *new std::map<std::tuple<int, int, cudaStream_t>, std::pair<unsigned long long, at::Tensor>>();
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
     C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
-    const auto key = std::make_tuple(which, static_cast<int>(like.get_device()), stream);
+    const WorkspaceKey key(which, static_cast<int>(like.get_device()), stream);
     const auto fresh = [&] { return at::zeros({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)); };
-    const std::lock_guard<std::mutex> guard(lock);
+    const std::lock_guard<std::mutex> guard(g_workspace_lock);
     if (status == cudaStreamCaptureStatusActive) {
-        auto &c = captured[key];
+        auto &c = g_captured_workspaces[key];
         if (!c.second.defined() || c.first != id || static_cast<size_t>(c.second.numel()) < bytes) c = {id, fresh()};
         return c.second;
     }
-    at::Tensor &t = kept[key];
+    at::Tensor &t = g_workspaces[key];
     if (!t.defined() || static_cast<size_t>(t.numel()) < bytes) t = fresh();
     return t;
+}
+
+// After a timeout on `device` (nothing in flight): the next calls there start on zeroed buffers.
+void reset_workspaces(int64_t device) {
+    const std::lock_guard<std::mutex> guard(g_workspace_lock);
+    for (auto it = g_workspaces.begin(); it != g_workspaces.end();)
+        it = std::get<1>(it->first) == device ? g_workspaces.erase(it) : std::next(it);
 }
 
 at::Tensor kv8_rope_append(const at::Tensor &qkv, int64_t n_heads, const at::Tensor &k, const at::Tensor &v,
@@ -401,6 +410,7 @@ TORCH_LIBRARY(lse, m) {
           "Tensor context_len, float scale) -> Tensor");
     m.def("kv8_paged_attention(Tensor q, Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor block_table, "
           "Tensor context_len, Tensor query_offset, Tensor q_start, Tensor q_len, float scale) -> Tensor");
+    m.def("reset_workspaces(int device) -> ()", &reset_workspaces);
     m.def("token_logprobs(Tensor logits, Tensor? tokens, int top_k) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 

@@ -632,7 +632,7 @@ def _device_index(device: int | torch.device | None) -> int:
 
 def device_status(device: int | torch.device | None = None, reset: bool = True) -> int:
     """Synchronize and read the device-side status (LSE_OK or LSE_ERR_DEVICE_TIMEOUT).  After a
-    timeout the decode-attention workspaces of that device are re-zeroed (the linear
+    timeout the attention workspaces of that device are re-zeroed (the linear
     workspaces need nothing: each call initialises its own)."""
     idx = _device_index(device)
     st = int(_lib.load().lse_device_status(idx, 1 if reset else 0))
@@ -640,4 +640,6 @@ def device_status(device: int | torch.device | None = None, reset: bool = True) 
         for (d, _), ws in _attn_ws.items():
             if d == idx:
                 ws.zero_()
+        if _torch_ops_loaded:  # the 8-bit cache's attentions: zeroed anew at their next calls
+            torch.ops.lse.reset_workspaces(idx)
     return st

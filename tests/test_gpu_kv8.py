@@ -461,3 +461,24 @@ def test_streams_and_graphs():
     eager = step()
     for a, b in zip(eager, held):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("q_len,offset", [([300, 5], [0, 900]), ([2000], [1000])])
+def test_paged_attention_timeout_reports_and_next_call_is_clean(q_len, offset):
+    """A wait limit of one cycle makes the kernel's waits give up: the status says so, and with the
+    limit back the same call on the same stream is right (its tensor memory was freed, its
+    workspace zeroed anew)."""
+    q, cache, table, context, off, start, n = _prompt(q_len, offset, 8, 2, 128, 16, torch.bfloat16, seed=31)
+    args = (q, cache, table, *[_i32(a) for a in (context, off, start, n)])
+    want = ops.kv8_paged_attention(*args)
+    assert ops.device_status() == _lib.LSE_OK
+    ops.set_wait_limit(1)
+    try:
+        ops.kv8_paged_attention(*args)  # the launch itself succeeds
+        assert ops.device_status() == _lib.LSE_ERR_DEVICE_TIMEOUT
+    finally:
+        ops.set_wait_limit(0)
+    got = ops.kv8_paged_attention(*args)
+    assert ops.device_status() == _lib.LSE_OK
+    rows = np.concatenate([np.arange(s, s + k) for s, k in zip(start, n)])
+    assert torch.equal(got[:, rows], want[:, rows])
