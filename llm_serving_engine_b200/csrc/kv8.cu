@@ -311,7 +311,7 @@ int lse_kv8_paged_attention(const void *q, int dtype, int64_t tokens, int64_t H,
     if ((rc = check_table(block_table, bt_stride, bt_cols, E, block_size))) return rc;
     if (tokens > INT32_MAX / 2) return LSE_ERR_UNSUPPORTED;
     {  // the kernel counts position tiles in 32 bits: items of 256 rows times the tiles of the longest context
-        const int64_t items = tokens * (H / H_kv) / kv8::PR_ROWS + E, tiles = bt_cols * block_size / kv8::PR_KEYS + 1;
+        const int64_t items = tokens * (H / H_kv) / kv8::PR_ROWS + E, tiles = bt_cols * block_size / kv8::PR_KEYS + 1 + kv8::PR_START;
         if (items * H_kv > INT32_MAX / 2 / tiles) return LSE_ERR_UNSUPPORTED;
     }
     if (!aligned(q, 16) || !aligned(o, 16) || q_stride_h % 8 || q_stride_m % 8 || o_stride_h % 8 || o_stride_m % 8 ||

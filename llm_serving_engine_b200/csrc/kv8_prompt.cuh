@@ -42,6 +42,10 @@ constexpr int PR_WARPS = 13;
 constexpr int PR_THREADS = PR_WARPS * 32;
 constexpr int PR_TABLES = 4;        // scale tables in flight
 constexpr int PR_SPLIT_TILES = 8;
+// What an item costs apart from its position tiles, in tiles: Q in, the first tile without overlap, the
+// output.  Runs are cut by this cost (us at 0 / 1 / 2 / 3 / 4 / 6: one prompt of 8192, 32 heads over 8,
+// 1118 / 1040 / 961 / 883 / 916 / 938; a mixed batch of 64 entries 229 / 182 / 167 / 168 / 174 / 179).
+constexpr int PR_START = 3;
 
 struct PromptWork {
     int *counters;  // [grid], as DecodeWork
@@ -92,19 +96,20 @@ struct PromptSchedule {
     __device__ __forceinline__ int entry_tiles() const {
         int n = 0;
 #pragma unroll 1
-        for (int k = 0; k < nq; ++k) n += tiles_of(context, offset, q_len, tok, k);
+        for (int k = 0; k < nq; ++k) n += PR_START + tiles_of(context, offset, q_len, tok, k);
         return n;
     }
     __device__ __forceinline__ bool next(const AttnParams &p, PromptSegment &s) {
         if (at >= end) return false;
         if (split) {
             const int n = tiles_of(context, offset, q_len, tok, i);
-            s.j0 = at - first;
-            s.j1 = min(end, first + n) - first;
+            if (end <= first + PR_START) return false;  // the item's first tile is the next CTA's
+            s.j0 = max(at - first - PR_START, 0);
+            s.j1 = min(end - first - PR_START, n);
             fill(s, n);
-            at = first + s.j1;
+            at = first + PR_START + s.j1;
             if (s.j1 == n) {  // the next item
-                first += n;
+                first += PR_START + n;
                 if (++i == nq) {
                     i = 0;
                     if (++kvh == p.H_kv) {
@@ -141,7 +146,7 @@ struct PromptSchedule {
         s.q_len = q_len;
         s.offset = offset;
         s.context = context;
-        s.item = first;
+        s.item = first + PR_START;
     }
     // CTA whose run holds a tile (split)
     __device__ __forceinline__ int cta_of(int tile) const {
@@ -308,7 +313,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             __syncthreads();
             items_all *= p.H_kv;
             tiles_all = base_tiles * p.H_kv;
-            sched.split = tiles_all >= PR_SPLIT_TILES * items_all;
+            sched.split = tiles_all >= (PR_SPLIT_TILES + PR_START) * items_all;
             sched.total = tiles_all;
             if (!sched.split) break;
             // no run shorter than SPLIT_TILES tiles
@@ -331,7 +336,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
             sched.kvh = (sched.at - s_found[1]) / s_found[2];
             sched.first = s_found[1] + sched.kvh * s_found[2];
 #pragma unroll 1
-            for (int n; sched.first + (n = PromptSchedule::tiles_of(sched.context, sched.offset, sched.q_len, sched.tok, sched.i)) <= sched.at; ++sched.i)
+            for (int n; sched.first + (n = PR_START + PromptSchedule::tiles_of(sched.context, sched.offset, sched.q_len, sched.tok, sched.i)) <= sched.at; ++sched.i)
                 sched.first += n;
         }
         if (lane == 0) s_sched[warp] = sched;
@@ -463,15 +468,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
                             over = __hgt(__hmax(__low2half(most), __high2half(most)), __float2half_rn(64.f));
                         } else {  // unseen: no weight; mute pages: values of 0
                             over = false;
+                            float f = 0.f, v = 0.f;
 #pragma unroll
                             for (int k = 0; k < 16; ++k) {
                                 float y[2];
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) {
+                                    if (!PAGED16 || (2 * k + h) % 16 == 0) {
+                                        f = sk[2 * k + h] * c;
+                                        v = sv[2 * k + h];
+                                    }
                                     const bool on = (seen >> (2 * k + h)) & 1u;
-                                    const float w = on ? ex2_approx(fmaf(__uint_as_float(sr[2 * k + h]), sk[2 * k + h] * c, -M)) : 0.f;
+                                    const float w = on ? ex2_approx(fmaf(__uint_as_float(sr[2 * k + h]), f, -M)) : 0.f;
                                     add[h] += w;
-                                    y[h] = on ? w * sv[2 * k + h] : 0.f;
+                                    y[h] = on ? w * v : 0.f;
                                     over |= y[h] > 64.f;
                                     if ((mute >> (2 * k + h)) & 1u) y[h] = 0.f;
                                 }
