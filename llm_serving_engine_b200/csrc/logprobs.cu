@@ -46,17 +46,23 @@ extern "C" int lse_token_logprobs(const void *logits, int dtype, int64_t M, int6
     p.V = static_cast<int>(V);
     p.k = static_cast<int>(top_k);
     // CTAs of a row: as many as are resident at once (3 an SM), as long as each of a CTA's warps has a group
+    // (rows of 128256: one row with 5 alternatives 9.6 us, 17.5 with one CTA; 64 with 20 18.4 against 36.9)
     const int step = 128 * static_cast<int>(16 / el);  // logits of one warp's loads
     p.group = step;
     p.cluster = 1;
-    while (p.cluster < logprobs::MAX_CLUSTER && 2 * M * p.cluster <= 3 * host::num_sms(dev) &&
+    // Too few groups (512 logits each) for so many alternatives: 16 bytes are one, in a single CTA (64 bf16 rows
+    // of 32000 with 128: 54 us against 2608 with groups of 512, all of whose logits would be candidates;
+    // 8192 with 20: 9.0 against 89)
+    const int64_t steps = (V + 16 + step - 1) / step;
+    const bool scarce = 8 * top_k > 7 * ((V + 16) / 512) && steps * 128 <= logprobs::FINE_GROUPS;
+    while (!scarce && p.cluster < logprobs::MAX_CLUSTER && 2 * M * p.cluster <= 3 * host::num_sms(dev) &&
            V > static_cast<int64_t>(p.cluster) * logprobs::WARPS * step)
         p.cluster *= 2;
     const int limit = (p.cluster > 1 ? 256 : logprobs::MAX_GROUPS) / 2;  // two maxima a group
     auto groups = [&] { return (V + 16 + static_cast<int64_t>(p.group) * p.cluster - 1) / (static_cast<int64_t>(p.group) * p.cluster); };
     while (groups() > limit) p.group *= 2;
     p.groups = static_cast<int>(groups());
-    p.fine = p.cluster == 1 && p.group == step && p.groups * 128 <= logprobs::MAX_GROUPS;
+    p.fine = p.cluster == 1 && p.group == step && p.groups * 128 <= (scarce ? logprobs::FINE_GROUPS : logprobs::MAX_GROUPS);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute pdl[1], attr[2];
     if (M * p.cluster > INT32_MAX) return LSE_ERR_UNSUPPORTED;

@@ -52,6 +52,13 @@ def test_against_the_oracle(M, V, k, dtype):
     assert ops.device_status() == _lib.LSE_OK
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,V,k", [(3, 8192, 20), (70, 9001, 33), (2, 32000, 128), (1, 37001, 128), (2, 50257, 128), (2, 66000, 128)])
+def test_more_alternatives_than_groups(M, V, k, dtype):
+    x, tokens = _logits(M, V, dtype, seed=11 * V + k)
+    _check(x, tokens, k)
+
+
 def test_leading_shape_and_no_tokens():
     x, tokens = _logits(6, 1000, torch.bfloat16, seed=1)
     _check(x.view(2, 3, 1000), tokens.view(2, 3), 4)
