@@ -19,7 +19,10 @@
 // decode step, the second time from registers).  q in warps of their own, a token's heads a few at a
 // time with its cos and sin in registers.  A lane holds two 16-byte runs of a row, a pair's
 // two sides, so that all loads and stores are vectors.  Bound by DRAM for prompts, by latency
-// for decode (one row per page).
+// for decode (one row per page; table, offsets, page scale and row are round trips one after another).
+// Measured with the read of the touched pages that follows: five chunks of up to 2048 tokens, 64 heads
+// of 128 over 8 (391 MB) 129 us, 3.0 TB/s; one token, or one of each of 64 sequences, 17 us through two
+// public calls, of which the GPU has 5.9 and 8.0.
 #pragma once
 
 #include <type_traits>

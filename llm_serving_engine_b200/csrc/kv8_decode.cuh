@@ -5,12 +5,16 @@
 //
 // A stream over the cache: 2 D bytes a position and KV head, shared by the G = H / H_kv query
 // heads.  What the kernel is shaped by:
-//   * The codes go from global memory straight into the registers of the warp MMA's row operand
-//     (m16n8k16): S^T = K Q^T has 16 positions as rows and the query heads as its 8 columns, and
-//     O^T += V^T P^T has 16 dims as rows.  The order of a contraction's index is free, so a thread's
-//     operand is made of 16-byte runs of a row: K row r0 (and r0 + 8), chunks q4 and q4 + 4; V rows
-//     2 q4, 2 q4 + 1 (+ 8), chunk r0 (r0 = lane / 4, q4 = lane % 4).  No shared memory, no barrier
-//     in the loop; the next tile's loads are in flight under the current one's arithmetic.
+//   * Each warp keeps a ring of tiles of 32 positions in shared memory, filled by 16-byte
+//     asynchronous copies and read by nobody else, so there is no barrier in the loop.  A group of
+//     lanes copies a whole row (a whole 128-byte line at D = 128: copying half lines for the lanes that
+//     use them doubled the traffic from L2), swizzled by 16-byte chunks.  2 stages at D = 128 and 3
+//     CTAs an SM hold 96 KB of copies in flight per SM; 4 stages, 2 CTAs or tiles of 16 were slower.
+//   * They feed the row operand of the warp MMA (m16n8k16): S^T = K Q^T has 16 positions as rows and
+//     the query heads as its 8 columns, and O^T += V^T P^T has 16 dims as rows.  The order of a
+//     contraction's index is free, so a thread's operand is made of 16-byte runs of a row: K row r0
+//     (and r0 + 8), chunks q4 and q4 + 4; V rows 2 q4, 2 q4 + 1 (+ 8), chunk r0 (r0 = lane / 4, q4 =
+//     lane % 4).  At most 8 query heads share a row: the tensor core is far from the bound.
 //   * int8 -> fp16 is exact: one byte permute puts a biased code under the exponent of 1024, one
 //     subtraction takes the bias off.  q is fp16 after an exact power-of-two scaling per head (bf16)
 //     or as it is; scores are fp32 sums of exact products.
@@ -23,6 +27,11 @@
 //     the device, so a ragged batch and a single long sequence fill the GPU alike, and the launch
 //     is the same for every batch.  A pair that several CTAs share is joined by the CTA that
 //     arrives last, in the order of the positions (deterministic); none waits for another.
+//
+// Bound by DRAM with many positions, by latency (page look-up, scales, copy, join: one round trip
+// each) with few.  Measured, KV heads of 128 dims in pages of 16: 64 sequences of 1 to 4096 positions, 32
+// heads over 8 (304 MB) 64.1 us, 4.74 TB/s; 8 of up to 65536, 64 heads over 8 (761 MB) 156 us, 4.87 TB/s
+// (a copy reaches 6.5); one of 1025 9.8 us.
 #pragma once
 
 #include "common.cuh"
@@ -93,7 +102,8 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t u) {
 }
 
 // PAGED8: block_size is a multiple of 8, so that 8 consecutive positions share a page and its scales;
-// otherwise every position looks its page up for itself.
+// otherwise every position looks its page up for itself (64 sequences of up to 4096 in pages of 16: 64.6 us,
+// 75.2 so; 8 of up to 65536: 159 and 183; alone with 1025 positions the two differ by the timer's step).
 template <int D, int G, typename T, bool PAGED8>
 __global__ void __launch_bounds__(DEC_THREADS, 3) decode_kernel(const AttnParams p, const DecodeWork w) {
     constexpr int U = 2;                // 16-position MMA rows of a tile

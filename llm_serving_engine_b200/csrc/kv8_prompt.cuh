@@ -21,7 +21,19 @@
 // The work, (entry, KV head, 256-row item) x position tiles laid end to end, is cut into equal runs
 // of tiles, one per SM, from the lengths on the device; items that several CTAs share are joined by the
 // last to arrive, in the order of the positions.  Where items are short (fewer than SPLIT_TILES tiles on
-// average) they are dealt whole instead: a joint costs more than it gains there.
+// average) they are dealt whole instead: a joint costs more than it gains there (a prompt of 512, 4 tiles at
+// most an item: 28.9 us whole, 53.3 cut; a prompt of 8192: 884 cut, 946 whole; the mixed batch below 168
+// cut, 214 whole).
+//
+// Bound by the chain S -> softmax -> P -> S of the two row tiles: for 256 rows x 128 positions the
+// products alone take 2060 cycles (67 a 128 x 128 x 16 step), the exponentials 2050 of the
+// special-function units, while a softmax tile takes 4500 to 5000 and its pair's turn about 7000.
+// Measured: a prompt of 8192, 32 heads of 128 over 8, 882 us, 623 TFLOP/s (38% of what a plain matrix
+// product reaches); 512 tokens 29.2 us (latency); 8 single tokens and 4 chunks of up to 700 after up
+// to 5000 positions, 32 heads of 64 over 4, 168 us.  S in halves of 64 positions with two buffers was
+// slower (1224 against 1117 at that step), as were S prefetched by 16 columns, out-of-line
+// roles, a converter with one copy of its code, and two threads a row (16 softmax warps at 80 registers, M
+// agreed between the two: 1089 us; 512: 36.8).
 #pragma once
 
 #include <climits>
@@ -44,7 +56,8 @@ constexpr int PR_TABLES = 4;        // scale tables in flight
 constexpr int PR_SPLIT_TILES = 8;
 // What an item costs apart from its position tiles, in tiles: Q in, the first tile without overlap, the
 // output.  Runs are cut by this cost (us at 0 / 1 / 2 / 3 / 4 / 6: one prompt of 8192, 32 heads over 8,
-// 1118 / 1040 / 961 / 883 / 916 / 938; a mixed batch of 64 entries 229 / 182 / 167 / 168 / 174 / 179).
+// 1118 / 1040 / 961 / 883 / 916 / 938; 8 single tokens and 4 chunks of up to 700 after up to 5000
+// positions, 32 heads of 64 over 4, 229 / 182 / 167 / 168 / 174 / 179).
 constexpr int PR_START = 3;
 
 struct PromptWork {
@@ -194,7 +207,8 @@ __device__ __forceinline__ uint32_t out2(float lo, float hi) {  // two elements 
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// PAGED16: block_size is a multiple of 16, so that 16 positions share a page and its scales.
+// PAGED16: block_size is a multiple of 16, so that 16 positions share a page and its scales (a prompt of 8192
+// in pages of 16: 884 us, 1491 with a look at the table for every position; 512: 29.1 and 35.5).
 template <int D, typename T, bool PAGED16>
 __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ PromptWork work, const int log_g) {
     using S = PromptSmem<D>;
@@ -733,8 +747,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const __grid_cons
     } else {
         // ==== the MMA issuer ==========================================================================
         // The whole warp runs this role and one elected lane issues: with warp-uniform control the
-        // descriptors stay in uniform registers (a branch on lane 0 around the role cost 130 cycles an
-        // MMA, whatever its size; elected, 101 from shared memory and 73 with P from tensor memory).
+        // descriptors stay in uniform registers, and unrolled the steps come every 67 cycles, the pipe's own
+        // pace at 128 x 128 x 16 (a branch on lane 0 around the role: 130 cycles a step, whatever its size).
         uint32_t elected;
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
         const bool lead = elected != 0;
