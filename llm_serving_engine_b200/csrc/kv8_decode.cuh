@@ -9,7 +9,7 @@
 //     asynchronous copies and read by nobody else, so there is no barrier in the loop.  A group of
 //     lanes copies a whole row (a whole 128-byte line at D = 128: copying half lines for the lanes that
 //     use them doubled the traffic from L2), swizzled by 16-byte chunks.  2 stages at D = 128 and 3
-//     CTAs an SM hold 96 KB of copies in flight per SM; 4 stages, 2 CTAs or tiles of 16 were slower.
+//     CTAs an SM are 192 KB of tiles an SM, read or on their way; 4 stages, 2 CTAs or tiles of 16 were slower.
 //   * They feed the row operand of the warp MMA (m16n8k16): S^T = K Q^T has 16 positions as rows and
 //     the query heads as its 8 columns, and O^T += V^T P^T has 16 dims as rows.  The order of a
 //     contraction's index is free, so a thread's operand is made of 16-byte runs of a row: K row r0
